@@ -381,6 +381,24 @@ int mp_decode_layer_window_ex(mp_simhash_t* s, mp_lsh_t* lsh, mp_attn_t* attn, m
                               int layer_id, const uint16_t* q, const int32_t* window_len, uint16_t* output,
                               float* max_value_expsum, int32_t* nnz_out, unsigned int flags, mp_stream_t stream);
 
+/* ---------------------------------------------------------------- whole prompts
+ * Exact causal attention over whole prompts packed one behind the other: what FlashInfer's prefill does for the reference
+ * in front of LSHSparseAttnServer.fill (models/attnserver.py:112-175), for any number of prompts in one launch.
+ *   q bf16 [num_tokens, H, D], k, v bf16 [num_tokens, Hkv, D] through their token and head strides (elements; slices of one
+ *   fused projection are used in place; dims contiguous), every address 16-byte aligned, token strides below 2^23;
+ *   cu_seqlens int32 [num_seqs + 1] (device): sequence b is the rows cu_seqlens[b] .. cu_seqlens[b + 1]; sequences may be
+ *   empty; rows in front of the first and behind the last sequence are not read and their outputs stay as they were;
+ *   output bf16 [num_tokens, H, D], lse f32 [num_tokens, H] (base-2 log-sum-exp, may be NULL), contiguous.
+ * Token i of a sequence sees its tokens 0 .. i; query head h reads kv head h / (H / Hkv).  head_dim 64 or 128; scale > 0.
+ * An infinity or NaN in a key or value reaches the rows that see it and no others.  Offsets that decrease or leave
+ * [0, num_tokens] are clamped (no access outside the tensors), the results are then unspecified.  Device pointers only, work
+ * is enqueued on `stream` of the current device; no state, no workspace: calls may overlap and be captured. */
+int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
+                        int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v, int64_t v_token_stride,
+                        int64_t v_head_stride, const int32_t* cu_seqlens, int num_seqs, int64_t num_tokens,
+                        int num_attention_heads, int num_key_value_heads, int head_dim, float scale, uint16_t* output,
+                        float* lse, mp_stream_t stream);
+
 /* ---------------------------------------------------------------- LSE merge
  * Replaces flashinfer.merge_state as called at models/attnserver.py:308 (base-2 LSEs):
  * v = (2^sa va + 2^sb vb) / 2^s, s = log2(2^sa + 2^sb).  va, vb, v bf16 [R, D]; sa, sb, s f32 [R]

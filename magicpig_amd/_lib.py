@@ -94,6 +94,7 @@ def lib() -> C.CDLL:
         "mp_decode_layer_window": ([p, p, p, p, i32, p, p, p, p, p, p], i32),
         "mp_decode_sparse_layer_ex": ([p, p, p, i32, p, p, p, p, C.c_uint, p], i32),
         "mp_decode_layer_window_ex": ([p, p, p, p, i32, p, p, p, p, p, C.c_uint, p], i32),
+        "mp_prompt_attention": ([p, i64, i64, p, i64, i64, p, i64, i64, p, i32, i64, i32, i32, i32, C.c_float, p, p, p], i32),
         "mp_merge_state": ([p, p, p, p, i32, i32, p, p, p], i32),
     }
     for name, (args, res) in sig.items():

@@ -1,0 +1,288 @@
+// attn_tile.h -- the tile arithmetic shared by the attention over whole prompts (prompt.hip) and over the paged
+// cache (paged.hip).
+//
+// Rows.  The query heads of one kv head read the same keys, so they share a tile: row r of a (sequence, kv head) is
+// head r % G of token r / G.  A tile of rows starts at a multiple of its height, a sequence of n tokens has n G rows.
+//
+// Mathematics.  For a row with visible keys 0 .. lim the kernels fold the tokens in once, tile by tile:
+//     s_j = q . k_j (f32 accumulation of exact bf16 products),  x_j = c s_j,  c = scale log2(e)
+//     m' = max(m, max_j x_j),  l' = 2^(m - m') l + sum_j 2^(x_j - m'),  o' = 2^(m - m') o + sum_j 2^(x_j - m') v_j
+// and end with o / l and the base-2 log-sum-exp m + log2 l.  m only moves when a tile's maximum lies more than
+// 8 above it (2^8 times larger weights change neither f32 sums nor the relative precision of a bf16 weight), so
+// most tiles rescale nothing.  m, l, o are f32; the weights 2^(x - m) are rounded to bf16 once, for the second
+// matrix product (relative error 2^-9 each, the rounding the output gets anyway); l sums them unrounded.
+//
+// Lanes.  Both products are v_mfma_f32_32x32x16_bf16.  The first computes S^T = K Q^T: lane l holds column
+// (row of q) l % 32 and, of 32 tokens, the 16 with (t >> 2) & 1 == l / 32.  So a row's maximum and sum are sums over a
+// lane's own registers and one exchange with lane l ^ 32, and its weights are, as they lie, the right-hand operand of
+// O^T = V^T P^T: the product's 16 inner indices may be any 16 tokens in any order as long as both operands agree, here
+// inner index 8 (l / 32) + j is token 8 (j / 4) + 4 (l / 32) + j % 4.  V^T comes out of the row-major tile in LDS
+// through ds_read_b64_tr_b16 (16 lanes read a 4 x 16 block and each gets a column of it).
+//
+// LDS.  Tile rows are 2 D bytes, 16-byte chunks.  Slot p of row r holds chunk p ^ key_swizzle(r) / p ^ value_swizzle(r): the 32
+// rows that one K read touches then lie in all banks evenly, and so do the 4 rows x 64 bytes of a transposed V read.
+// (The DMA into LDS writes lane after lane: the permutation is made on the global addresses.)
+#pragma once
+#include "common.h"
+
+namespace mp {
+
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
+#define MP_LDS __attribute__((address_space(3)))
+#define MP_GLOBAL __attribute__((address_space(1)))
+
+constexpr int TILE_TOKENS = 64;         // tokens staged at a time
+constexpr float NEG_INF = -__builtin_inff();
+constexpr float LAZY_MAX = 8.f;         // see above: how far a maximum may lie above m before m follows
+
+template <int D>
+__device__ __forceinline__ int key_swizzle(int row) { return D == 128 ? (row & 15) : ((row >> 1) & 7); }
+template <int D>
+__device__ __forceinline__ int value_swizzle(int row) { return D == 128 ? ((row & 3) << 2) : (((row >> 1) & 1) << 2); }
+
+// max / sum with the lane 32 away; both get the result
+__device__ __forceinline__ float halves_max(float x) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    bf16x2 r;
+    r[0] = (__bf16)a;
+    r[1] = (__bf16)b;
+    return __builtin_bit_cast(uint32_t, r);
+}
+
+// 16 bytes of global memory per lane straight into LDS at `l` + 16 * lane (l wave-uniform)
+__device__ __forceinline__ void dma16(const char* g, char* l) {
+    __builtin_amdgcn_global_load_lds((const MP_GLOBAL void*)g, (MP_LDS void*)l, 16, 0, 0);
+}
+// every outstanding load and LDS write of this wave has landed, then the workgroup meets
+__device__ __forceinline__ void tile_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// What a wave keeps of its 32 rows.
+template <int D>
+struct RowState {
+    bf16x8 q[D / 16];      // right-hand operand of S^T: row l % 32, dims 16 s + 8 (l / 32) ..
+    f32x16 o[D / 32];      // O^T: dims 32 i + 8 (r / 4) + 4 (l / 32) + r % 4
+    float m, l;            // running maximum (base 2) of both halves; this half's share of the sum
+};
+
+template <int D>
+__device__ __forceinline__ void load_rows(RowState<D>& st, const uint16_t* q) {     // q: this lane's row
+    const int h = lane_id() >> 5;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) st.q[s] = *reinterpret_cast<const bf16x8*>(q + 16 * s + 8 * h);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st.o[i][r] = 0.f;
+    st.m = NEG_INF;
+    st.l = 0.f;
+}
+
+// This lane's left-hand operand of O^T: dims 32 i + l % 32, tokens 16 t + 8 (j / 4) + 4 (l / 32) + j % 4
+template <int D>
+__device__ __forceinline__ bf16x8 read_v(const char* vt, int i, int t) {
+    const int l = lane_id(), r = (l & 15) >> 2;
+    const int swz = D == 128 ? (i ^ r) : (i ^ (r >> 1));
+    const char* p = vt + (4 * (l >> 5) + r) * (2 * D) + swz * 64 + ((l >> 4) & 1) * 32 + (l & 3) * 8 + t * 16 * (2 * D);
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MP_LDS s16x4*)(p));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MP_LDS s16x4*)(p + 8 * (2 * D)));
+    typedef __attribute__((ext_vector_type(8))) short s16x8;
+    const s16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(bf16x8, v);
+}
+
+// A masked tile may hold values that a row must not see, and 0 times an infinity is NaN.  Product with zeros first:
+// finite values give 0, anything else NaN.
+template <int D, int SUB>
+__device__ __forceinline__ bool tile_has_nonfinite(const char* vt) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    bf16x8 zero;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) zero[j] = (__bf16)0.f;
+#pragma unroll
+    for (int t = 0; t < 2 * SUB; ++t)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(read_v<D>(vt, i, t), zero, acc, 0, 0, 0);
+    const float s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+    asm volatile("" ::: "memory");       // what follows reads the tile again: these 64 registers are not kept for it
+    return __ballot(!(s == 0.f)) != 0;
+}
+
+// ... and where a masked tile does, its finite values alone go into the product (0 for the others) ...
+// 0xffff in the halves of w that are not finite
+__device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
+    return ((((w & 0x7f807f80u) + 0x00800080u) >> 15) & 0x00010001u) * 0xffffu;
+}
+__device__ __forceinline__ bf16x8 finite_only(bf16x8 x) {
+    u32x4 v = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] &= ~nonfinite_halves(v[j]);
+    return __builtin_bit_cast(bf16x8, v);
+}
+// ... and the others are counted per row and dim over the tokens the row sees -- +inf, -inf and NaN as 1, 2^7 and 2^14 of
+// one exact product, at most 64 of each -- and join as what a sum over them is.  Rare: one block at a time, few registers.
+template <int D, int SUB>
+__device__ __forceinline__ void add_nonfinite(f32x16 (&o)[D / 32], const char* vt, int lim) {
+    const int h = lane_id() >> 5;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+        f32x16 cnt;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) cnt[r] = 0.f;
+        asm volatile("" : "+v"(lim));        // (what depends on it is computed again, not kept in 16 registers)
+#pragma unroll
+        for (int t = 0; t < 2 * SUB; ++t) {
+            __builtin_amdgcn_sched_barrier(0);
+            const u32x4 v = __builtin_bit_cast(u32x4, read_v<D>(vt, i, t));
+            u32x4 odd, see;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t nan = ((((v[j] & 0x007f007fu) + 0x007f007fu) >> 7) & 0x00010001u) * 0xffffu;   // given not finite
+                const uint32_t neg = ((v[j] >> 15) & 0x00010001u) * 0xffffu;
+                odd[j] = nonfinite_halves(v[j]) &
+                         ((nan & 0x46804680u) | (~nan & ((neg & 0x43004300u) | (~neg & 0x3f803f80u))));
+                const int tok = 16 * t + 8 * (j >> 1) + 4 * h + 2 * (j & 1);
+                see[j] = ((uint32_t)((tok - lim - 1) >> 31) & 0x3f80u) | ((uint32_t)((tok - lim) >> 31) & 0x3f800000u);
+            }
+            cnt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, odd), __builtin_bit_cast(bf16x8, see),
+                                                          cnt, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int n = (int)cnt[r];
+            const float pos = (n & 127) ? __builtin_inff() : 0.f, neg = (n >> 7 & 127) ? NEG_INF : 0.f;
+            o[i][r] += n >> 14 ? __builtin_nanf("") : pos + neg;
+        }
+    }
+}
+
+// Fold SUB * 32 tokens (K rows at kt, V rows at vt in LDS) into the wave's rows.  MASK: only tokens <= lim (relative to the
+// tile, per lane) are visible to the lane's row.
+template <int D, int SUB, bool MASK>
+__device__ __forceinline__ void fold_tile(RowState<D>& st, const char* kt, const char* vt, float c, int lim) {
+    const int l = lane_id(), h = l >> 5, row = l & 31;
+    f32x16 s[SUB];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (32 * u + row) * (2 * D) + (((2 * k + h) ^ key_swizzle<D>(row)) << 4));
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, st.q[k], s[u], 0, 0, 0);
+        }
+    if (MASK) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (32 * u + 8 * (r >> 2) + 4 * h + (r & 3) > lim) s[u][r] = NEG_INF;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    top = halves_max(top) * c;
+    if (__ballot(top > st.m + LAZY_MAX)) {               // (-inf + 8 = -inf: a row's first visible tile always enters)
+        const float m = fmaxf(st.m, top);
+        const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
+        st.m = m;
+        st.l *= f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st.o[i][r] *= f;
+    }
+    const float off = st.m == NEG_INF ? 0.f : st.m;      // nothing seen yet: every weight below is 2^-inf = 0
+    bf16x8 p[2 * SUB];
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], c, -off));
+            sum += w;
+            p[2 * u + (r >> 3)][r & 7] = (__bf16)w;
+        }
+    st.l += sum;
+    const bool odd = MASK && tile_has_nonfinite<D, SUB>(vt);
+#pragma unroll
+    for (int t = 0; t < 2 * SUB; ++t) {
+        if (MASK) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            bf16x8 v = read_v<D>(vt, i, t);
+            if (MASK && odd) v = finite_only(v);
+            st.o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[t], st.o[i], 0, 0, 0);
+        }
+    }
+    if (MASK && odd) add_nonfinite<D, SUB>(st.o, vt, lim);
+}
+
+// Which sequence and which of its tiles a slot is.  Sequence b of rows cu[b] G .. cu[b + 1] G owns the slots from
+// floor(cu[b] G / BM) + b on: at least as many as it has tiles, for every split of the rows, so the grid needs
+// no list of tiles made beforehand -- floor(T G / BM) + B slots, at most B of them empty.  All lanes return the same.
+struct TileOf {
+    int seq;         // -1: no such sequence
+    int start, n;    // its first row of q (token) and its tokens
+    int row0;        // the tile's first row inside the sequence
+};
+template <int BM>
+__device__ __forceinline__ TileOf find_tile(const int32_t* __restrict__ cu, int B, int T, int G, int slot) {
+    auto first = [&](int i) { return (int)(((int64_t)min(max(cu[i], 0), T) * G) / BM) + i; };
+    int cnt = 0;
+    for (int base = 0; base < B; base += WAVE) {
+        const int i = base + lane_id();
+        cnt += __popcll(__ballot(i < B && first(min(i, B - 1)) <= slot));
+    }
+    TileOf t;
+    t.seq = -1;
+    t.start = t.n = t.row0 = 0;
+    const int b = __builtin_amdgcn_readfirstlane(cnt) - 1;
+    if (b < 0) return t;
+    const int tile = slot - first(b);
+    t.start = min(max(cu[b], 0), T);
+    t.n = min(max(cu[b + 1], 0), T) - t.start;
+    if (tile < 0 || t.n <= 0 || (int64_t)tile * BM >= (int64_t)t.n * G) return t;
+    t.row0 = tile * BM;
+    t.seq = b;
+    return t;
+}
+
+// Base-2 log-sum-exp of sum l over 2^m: -inf of nothing, +inf where a logit was (its weights are NaN, as inf - inf is).
+__device__ __forceinline__ float log_sum(float m, float l) {
+    return l == 0.f ? NEG_INF : m == __builtin_inff() ? m : m + __builtin_amdgcn_logf(l);
+}
+
+// The wave's rows as they leave: normalised, bf16, with the base-2 log-sum-exp; a row that saw nothing is 0 and -inf.
+template <int D>
+__device__ __forceinline__ void store_rows(const RowState<D>& st, uint16_t* out, float* lse) {     // this lane's row
+    const int h = lane_id() >> 5;
+    const float l = halves_sum(st.l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            u32x2 w;
+            w[0] = pack_bf16(st.o[i][4 * g] * inv, st.o[i][4 * g + 1] * inv);
+            w[1] = pack_bf16(st.o[i][4 * g + 2] * inv, st.o[i][4 * g + 3] * inv);
+            *reinterpret_cast<u32x2*>(out + 32 * i + 8 * g + 4 * h) = w;
+        }
+    if (lse != nullptr && h == 0) *lse = log_sum(st.m, l);
+}
+
+}  // namespace mp

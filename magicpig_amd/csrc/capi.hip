@@ -1713,6 +1713,40 @@ int mp_decode_layer_window_ex(mp_simhash_t* s, mp_lsh_t* lsh, mp_attn_t* attn, m
                         (hipStream_t)stream, "mp_decode_layer_window_ex");
 }
 
+// =================================================================== whole prompts
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool row_strides_ok(int64_t token, int64_t head) {
+    return token >= 0 && head >= 0 && token % 8 == 0 && head % 8 == 0 && token < (1 << 23);
+}
+static bool attention_scale_ok(float scale) { return scale > 0.f && scale < __builtin_inff(); }
+constexpr float LOG2E = 1.4426950408889634f;
+
+int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
+                        int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v, int64_t v_token_stride,
+                        int64_t v_head_stride, const int32_t* cu_seqlens, int num_seqs, int64_t num_tokens,
+                        int num_attention_heads, int num_key_value_heads, int head_dim, float scale, uint16_t* output,
+                        float* lse, mp_stream_t stream) {
+    const int H = num_attention_heads, Hkv = num_key_value_heads;
+    MP_REQUIRE(head_dim == 64 || head_dim == 128, MP_ERR_UNSUPPORTED, "mp_prompt_attention: head_dim must be 64 or 128");
+    MP_REQUIRE(Hkv >= 1 && H >= Hkv && H % Hkv == 0, MP_ERR_INVALID, "mp_prompt_attention: bad head counts");
+    MP_REQUIRE(num_seqs >= 1 && num_tokens >= 0, MP_ERR_INVALID, "mp_prompt_attention: bad sequence or token count");
+    MP_REQUIRE(attention_scale_ok(scale), MP_ERR_INVALID, "mp_prompt_attention: scale must be finite and above 0");
+    if (num_tokens == 0) return MP_OK;
+    MP_REQUIRE(q && k && v && cu_seqlens && output, MP_ERR_INVALID, "mp_prompt_attention: null argument");
+    MP_REQUIRE(row_strides_ok(q_token_stride, q_head_stride) && row_strides_ok(k_token_stride, k_head_stride) &&
+                   row_strides_ok(v_token_stride, v_head_stride),
+               MP_ERR_INVALID, "mp_prompt_attention: strides must be multiples of 8 elements, token strides below 2^23");
+    MP_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(output), MP_ERR_INVALID,
+               "mp_prompt_attention: q, k, v and output must be 16-byte aligned");
+    MP_REQUIRE(num_tokens <= (1ll << 30) / (H / Hkv) && prompt_grid(num_tokens, num_seqs, H / Hkv, Hkv) < (1ll << 31) - 1,
+               MP_ERR_UNSUPPORTED, "mp_prompt_attention: more rows than one launch can number");
+    MP_HIP_CHECK(launch_prompt_attention(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v,
+                                         v_token_stride, v_head_stride, cu_seqlens, num_seqs, (int)num_tokens, H, Hkv,
+                                         head_dim, scale * LOG2E, output, lse, (hipStream_t)stream));
+    return MP_OK;
+}
+
 // =================================================================== LSE merge
 
 int mp_merge_state(const uint16_t* va, const float* sa, const uint16_t* vb, const float* sb, int R,

@@ -1,11 +1,11 @@
-// capi_launchers.h -- the kernels' host launchers (simhash.hip, lsh.hip, attention.hip) as the C ABI's entry points call them
+// capi_launchers.h -- the kernels' host launchers (simhash.hip, lsh.hip, attention.hip, prompt.hip) as the C ABI's entry points call them
 // (one of the pieces capi.hip is made of: included there, once, in this order; not a header for other translation units)
 #pragma once
 
 namespace mp {
 
 
-// ---- kernels' host launchers (simhash.hip, lsh.hip, attention.hip)
+// ---- kernels' host launchers (simhash.hip, lsh.hip, attention.hip, prompt.hip)
 int simhash_padded_cols(int K, int L);
 int simhash_supported(int D, int K);
 hipError_t launch_simhash_prepare(const uint16_t*, int, int, int, uint16_t*, uint16_t*, float*, hipStream_t);
@@ -67,6 +67,10 @@ hipError_t launch_merge_state(const uint16_t*, const float*, const uint16_t*, co
                               int, uint16_t*, float*, hipStream_t);
 hipError_t launch_attn_append(const uint16_t*, const uint16_t*, const int32_t*, int, const uint16_t*, int, int, int, int64_t,
                               uint16_t*, float*, unsigned int*, int*, hipStream_t);
+int64_t prompt_grid(int64_t T, int B, int G, int Hkv);
+hipError_t launch_prompt_attention(const uint16_t*, int64_t, int64_t, const uint16_t*, int64_t, int64_t, const uint16_t*,
+                                   int64_t, int64_t, const int32_t*, int, int, int, int, int, float, uint16_t*, float*,
+                                   hipStream_t);
 bool lsh_hash_only_supported(int L);
 hipError_t launch_attn_ticket_check(int*, int, int*, hipStream_t);
 hipError_t launch_relay(const void*, void*, size_t, hipStream_t);

@@ -1,0 +1,86 @@
+// prompt.hip -- causal attention over whole prompts packed one behind the other, query heads in groups.
+//
+// A workgroup owns 128 rows (see attn_tile.h: a row is one query head of one token, the G heads of a kv head
+// side by side) of one (sequence, kv head) and walks the sequence's keys in tiles of 64 tokens, two buffers in LDS:
+// while tile j is folded in, the DMA engine fetches tile j + 1.  Its four waves hold 32 rows each.
+#include "attn_tile.h"
+
+namespace mp {
+
+struct PromptArgs {
+    const uint16_t *q, *k, *v;
+    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;     // strides of token and head, elements
+    const int32_t* cu;
+    int B, T, H, Hkv, G, slots;
+    float c;
+    uint16_t* out;
+    float* lse;
+};
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void prompt_attention_kernel(const PromptArgs a) {
+    constexpr int BM = 128, CPR = D / 8, PASSES = TILE_TOKENS * CPR / 256, KB = TILE_TOKENS * 2 * D;
+    __shared__ __attribute__((aligned(1024))) char lds[2][2][KB];      // [buffer][K, V]
+    // heads fastest: with 8 kv heads the workgroups of one head meet in one XCD's L2; longest rows of a sequence first
+    const int head = blockIdx.x % a.Hkv;
+    const TileOf t = find_tile<BM>(a.cu, a.B, a.T, a.G, a.slots - 1 - (int)(blockIdx.x / a.Hkv));
+    if (t.seq < 0) return;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+    const int rows = t.n * a.G;
+
+    const int wrow = t.row0 + 32 * w;                                   // the wave's first row
+    const int row = min(wrow + (l & 31), rows - 1);
+    const int tok = row / a.G, h = head * a.G + row % a.G;              // (row: the query's position in its sequence)
+    RowState<D> st;
+    load_rows<D>(st, a.q + (int64_t)(t.start + tok) * a.q_st + (int64_t)h * a.q_sh);
+
+    const int tiles = min(t.row0 + BM - 1, rows - 1) / a.G / TILE_TOKENS + 1;
+    const int whole = (t.row0 / a.G + 1) / TILE_TOKENS;                 // tiles that every row sees whole
+    const int seen = wrow < rows ? min(wrow + 31, rows - 1) / a.G / TILE_TOKENS + 1 : 0;    // tiles that the wave's rows see any of
+
+    const char* kb = reinterpret_cast<const char*>(a.k + (int64_t)t.start * a.k_st + (int64_t)head * a.k_sh);
+    const char* vb = reinterpret_cast<const char*>(a.v + (int64_t)t.start * a.v_st + (int64_t)head * a.v_sh);
+    const uint32_t kst = (uint32_t)a.k_st * 2, vst = (uint32_t)a.v_st * 2;
+    auto stage = [&](int tile) {
+        const char* kt = kb + (int64_t)tile * TILE_TOKENS * kst;
+        const char* vt = vb + (int64_t)tile * TILE_TOKENS * vst;
+        const int last = t.n - 1 - tile * TILE_TOKENS;                  // behind the end: the last token again, masked
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int idx = i * 256 + (int)threadIdx.x, r = idx / CPR, p = idx % CPR;
+            const uint32_t s = (uint32_t)min(r, last);
+            dma16(kt + (s * kst + ((p ^ key_swizzle<D>(r)) << 4)), lds[tile & 1][0] + (i * 256 + w * 64) * 16);
+            dma16(vt + (s * vst + ((p ^ value_swizzle<D>(r)) << 4)), lds[tile & 1][1] + (i * 256 + w * 64) * 16);
+        }
+    };
+    stage(0);
+    int j = 0;
+    for (; j < whole; ++j) {
+        tile_barrier();                                                 // tile j is there, tile j - 1 no longer read
+        if (j + 1 < tiles) stage(j + 1);
+        if (wrow < rows) fold_tile<D, 2, false>(st, lds[j & 1][0], lds[j & 1][1], a.c, 0);
+    }
+    for (; j < tiles; ++j) {
+        tile_barrier();
+        if (j + 1 < tiles) stage(j + 1);
+        if (j < seen) fold_tile<D, 2, true>(st, lds[j & 1][0], lds[j & 1][1], a.c, tok - j * TILE_TOKENS);
+    }
+    if (wrow + (l & 31) >= rows) return;
+    const int64_t orow = (int64_t)(t.start + tok) * a.H + h;
+    store_rows<D>(st, a.out + orow * D, a.lse ? a.lse + orow : nullptr);
+}
+
+int64_t prompt_grid(int64_t T, int B, int G, int Hkv) { return (T * G / 128 + B) * Hkv; }
+
+hipError_t launch_prompt_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, const uint16_t* k, int64_t k_st,
+                                   int64_t k_sh, const uint16_t* v, int64_t v_st, int64_t v_sh, const int32_t* cu, int B,
+                                   int T, int H, int Hkv, int D, float c, uint16_t* out, float* lse, hipStream_t st) {
+    const int G = H / Hkv;
+    const PromptArgs a{q, k, v, q_st, q_sh, k_st, k_sh, v_st, v_sh, cu, B, T, H, Hkv, G, (int)((int64_t)T * G / 128 + B), c, out, lse};
+    const dim3 grid((unsigned)prompt_grid(T, B, G, Hkv));
+    if (D == 128) prompt_attention_kernel<128><<<grid, 256, 0, st>>>(a);
+    else prompt_attention_kernel<64><<<grid, 256, 0, st>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace mp

@@ -1,0 +1,65 @@
+"""`prompt_attention` -- exact causal attention over whole prompts packed one behind the other, over the gfx950 C ABI
+(mp_prompt_attention).  The role of FlashInfer's prefill in front of the reference's LSHSparseAttnServer.fill
+(models/attnserver.py:112-175), for any number of prompts in one launch."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib as L
+
+
+def rows_strides(t: torch.Tensor, heads: int, head_dim: int, name: str):
+    """Checks a bf16 CUDA tensor [tokens, heads, head_dim] whose dims are contiguous; returns its token and head stride
+    (those of an axis of length 1, which torch leaves arbitrary, as if it were contiguous)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if t.dtype is not torch.bfloat16:
+        raise TypeError(f"{name}: expected dtype {torch.bfloat16}, got {t.dtype}")
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
+        raise ValueError(f"{name}: expected shape (tokens, {heads}, {head_dim}), got {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    if t.stride(2) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    head = t.stride(1) if heads > 1 else head_dim
+    return (t.stride(0) if t.shape[0] > 1 else heads * head_dim), head
+
+
+def same_device(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: on {t.device}, expected {device}")
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float | None = None,
+                     out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
+    """q bf16 [T, H, D]; k, v bf16 [T, Hkv, D] (any token / head strides that are multiples of 8 elements: slices of one
+    fused projection go in as they are); cu_seqlens int32 [B + 1]: sequence b is the rows cu_seqlens[b] .. cu_seqlens[b + 1].
+    Returns (out bf16 [T, H, D], lse f32 [T, H], base 2): token i of a sequence attends to its tokens 0 .. i, query head h to
+    kv head h // (H // Hkv).  scale: default head_dim ** -0.5.  Rows outside every sequence are not written: give `out` /
+    `lse` where their contents matter.  head_dim 64 or 128.  Runs on torch's current stream of q's device."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise ValueError("q: expected a tensor [tokens, heads, head_dim]")
+    T, H, D = q.shape
+    if not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise ValueError("k: expected a tensor [tokens, heads, head_dim]")
+    Hkv = k.shape[1]
+    qs = rows_strides(q, H, D, "q")
+    ks, vs = rows_strides(k, Hkv, D, "k"), rows_strides(v, Hkv, D, "v")
+    if k.shape[0] != T or v.shape[0] != T:
+        raise ValueError(f"k, v: expected {T} tokens, got {k.shape[0]} and {v.shape[0]}")
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+        raise ValueError("cu_seqlens: expected a tensor [sequences + 1]")
+    L.expect(cu_seqlens, torch.int32, cu_seqlens.shape, "cu_seqlens")
+    if out is None:
+        out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
+    if lse is None:
+        lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
+    L.expect(out, torch.bfloat16, (T, H, D), "out")
+    L.expect(lse, torch.float32, (T, H), "lse")
+    same_device(q.device, k=k, v=v, cu_seqlens=cu_seqlens, out=out, lse=lse)
+    with torch.cuda.device(q.device):                    # no handle: launch where the data is
+        L.check(L.lib().mp_prompt_attention(
+            L.ptr(q), *qs, L.ptr(k), *ks, L.ptr(v), *vs, L.ptr(cu_seqlens), cu_seqlens.shape[0] - 1, T, H, Hkv, D,
+            D ** -0.5 if scale is None else float(scale), L.ptr(out), L.ptr(lse), L.current_stream(q)))
+    return out, lse

@@ -1,0 +1,155 @@
+"""prompt_attention (mp_prompt_attention) against 64 bits: lengths, head groups, strides, masked infinities, rows outside the
+sequences, streams and graphs; its refusals (CPU)."""
+import pytest
+import torch
+
+import attention64
+import magicpig_amd as mp
+from magicpig_amd import _lib as L
+
+
+def packed(lens, H, Hkv, D, seed=0, before=0, behind=0):
+    g = torch.Generator().manual_seed(seed)
+    T = before + sum(lens) + behind
+    q = (torch.randn((T, H, D), generator=g) * 1.5).bfloat16().cuda()
+    k = (torch.randn((T, Hkv, D), generator=g) + 2 * torch.randn((1, Hkv, D), generator=g)).bfloat16().cuda()
+    v = torch.randn((T, Hkv, D), generator=g).bfloat16().cuda()
+    cu = torch.tensor([before] + [before + sum(lens[:i + 1]) for i in range(len(lens))], dtype=torch.int32).cuda()
+    return q, k, v, cu
+
+
+def compare(q, k, v, cu, out, lse, scale=None):
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    ends = cu.tolist()
+    for a, b in zip(ends, ends[1:]):
+        if b > a:
+            o, t, z, zt = attention64.attend(q[a:b], k[a:b], v[a:b], scale, torch.arange(b - a))
+            attention64.check(out[a:b], o, t, f"out of rows {a}..{b}")
+            attention64.check(lse[a:b], z, zt, f"lse of rows {a}..{b}")
+
+
+LENS = [[1], [2], [31], [32, 33], [63, 64, 65], [127, 128, 129], [0, 5, 0, 0, 7, 0], [1] * 70, [300, 1, 1000], [2049]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,Hkv", [(4, 4), (8, 2), (7, 1), (6, 2), (64, 2)])
+@pytest.mark.parametrize("lens", LENS, ids=lambda x: "x".join(map(str, x[:6])))
+def test_against_64_bits(lens, H, Hkv, D):
+    q, k, v, cu = packed(lens, H, Hkv, D, seed=H + D)
+    out, lse = mp.prompt_attention(q, k, v, cu)
+    compare(q, k, v, cu, out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_strided_inputs_and_scale(D):
+    lens, H, Hkv = [70, 3, 200], 8, 2
+    q, k, v, cu = packed(lens, H, Hkv, D, seed=5)
+    qkv = torch.cat([q, k, v], dim=1)
+    want = mp.prompt_attention(q, k, v, cu, scale=0.3)
+    compare(q, k, v, cu, *want, scale=0.3)
+    fused = mp.prompt_attention(qkv[:, :H], qkv[:, H:H + Hkv], qkv[:, H + Hkv:], cu, scale=0.3)
+    heads_first = mp.prompt_attention(*(x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)), cu, scale=0.3)
+    for got in (fused, heads_first):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_rows_outside_the_sequences_stay():
+    q, k, v, cu = packed([40, 90], 8, 2, 128, seed=6, before=3, behind=50)
+    out, lse = torch.full_like(q, 7.0), torch.full((q.shape[0], 8), -3.0, device="cuda")
+    mp.prompt_attention(q, k, v, cu, out=out, lse=lse)
+    compare(q, k, v, cu, out, lse)
+    for a, b in ((0, 3), (133, q.shape[0])):
+        assert bool((out[a:b] == 7.0).all()) and bool((lse[a:b] == -3.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_nonfinite_tokens_reach_only_rows_that_see_them(bad, D):
+    q, k, v, cu = packed([150, 77], 8, 2, D, seed=7)
+    v[100, 1, 5] = bad
+    v[149, 0] = bad
+    k[150 + 76, 0, 3] = bad
+    v[150 + 70, 1, D - 1] = -bad
+    v[150 + 71, 1, D - 1] = bad
+    out, lse = mp.prompt_attention(q, k, v, cu)
+    compare(q, k, v, cu, out, lse)
+    assert bool(torch.isfinite(out[:100]).all()) and bool(torch.isfinite(out[150:220]).all())
+
+
+@pytest.mark.gpu
+def test_peaked_and_flat_rows():
+    """Logits of thousands next to zeros: the maximum moves far and late, weights underflow."""
+    q, k, v, cu = packed([500], 4, 2, 128, seed=8)
+    q[100:200] *= 100
+    k[300] *= 60
+    q[400:] = 0
+    out, lse = mp.prompt_attention(q, k, v, cu)
+    compare(q, k, v, cu, out, lse)
+
+
+@pytest.mark.gpu
+def test_captured_on_a_side_stream_and_replayed():
+    q, k, v, cu = packed([130, 5, 61], 8, 2, 128, seed=9)
+    out, lse = torch.empty_like(q), torch.empty((q.shape[0], 8), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mp.prompt_attention(q, k, v, cu, out=out, lse=lse)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mp.prompt_attention(q, k, v, cu, out=out, lse=lse)
+    for step in range(3):
+        q2, k2, v2, cu2 = packed([100 - step, 31, 65 + step], 8, 2, 128, seed=20 + step)
+        for a, b in ((q, q2), (k, k2), (v, v2), (cu, cu2)):
+            a.copy_(b)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        again = mp.prompt_attention(q, k, v, cu)
+        assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+        compare(q, k, v, cu, out, lse)
+
+
+@pytest.mark.gpu
+def test_empty_inputs():
+    q, k, v, cu = packed([0, 0], 8, 2, 128)
+    out, lse = mp.prompt_attention(q, k, v, cu)
+    assert out.shape == (0, 8, 128) and lse.shape == (0, 8)
+
+
+# ---------------------------------------------------------------- refusals: nothing reaches the GPU
+GOOD = dict(q=1 << 20, qt=1024, qh=128, k=1 << 20, kt=256, kh=128, v=1 << 20, vt=256, vh=128, cu=1 << 20, seqs=2, tokens=10,
+            H=8, Hkv=2, D=128, scale=0.1, out=1 << 20, lse=1 << 20, stream=None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(D=96), 5), (dict(D=256), 5), (dict(H=7), 1), (dict(H=1), 1), (dict(Hkv=0), 1), (dict(seqs=0), 1), (dict(tokens=-1), 1),
+    (dict(scale=0.0), 1), (dict(scale=-1.0), 1), (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1),
+    (dict(q=None), 1), (dict(k=None), 1), (dict(v=None), 1), (dict(cu=None), 1), (dict(out=None), 1),
+    (dict(q=(1 << 20) + 2), 1), (dict(k=(1 << 20) + 8), 1), (dict(v=(1 << 20) + 4), 1), (dict(out=(1 << 20) + 8), 1),
+    (dict(qt=1020), 1), (dict(kh=12), 1), (dict(vt=-256), 1), (dict(vt=1 << 23), 1), (dict(tokens=1 << 29), 5),
+    (dict(seqs=(1 << 31) - 1), 5)])
+def test_refusals_of_the_c_entry(change, code):
+    a = {**GOOD, **change}
+    assert L.lib().mp_prompt_attention(*(a[n] for n in GOOD)) == code
+    assert b"mp_prompt_attention" in L.lib().mp_last_error()
+
+
+def test_refusals_of_the_python_entry():
+    x = torch.zeros((4, 8, 128), dtype=torch.bfloat16)
+    kv = torch.zeros((4, 2, 128), dtype=torch.bfloat16)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        mp.prompt_attention(x, kv, kv, cu)
+    with pytest.raises(TypeError, match="dtype"):
+        mp.prompt_attention(x.float(), kv, kv, cu)
+    with pytest.raises(ValueError, match="shape"):
+        mp.prompt_attention(x.cuda() if torch.cuda.is_available() else x, kv[:, :, :64], kv, cu)
+    with pytest.raises(ValueError, match="q:"):
+        mp.prompt_attention(x[0], kv, kv, cu)
