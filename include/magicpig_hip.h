@@ -53,9 +53,13 @@ extern "C" {
 #define MP_DTYPE_BF16 0
 #define MP_DTYPE_F32 1
 
+#define MP_KV_BF16 0 /* rows as they come */
+#define MP_KV_E4M3 1 /* e4m3 codes, one power of two per row */
+
 typedef struct mp_lsh mp_lsh_t;         /* replaces class LSH                    (library/lsh/lsh.h:14-43) */
 typedef struct mp_attn mp_attn_t;       /* replaces class SparseAttentionServer  (library/sparse_attention/sparse_attention.h:14-52) */
 typedef struct mp_simhash mp_simhash_t; /* replaces hash_func + binary_pack      (models/attnserver.py:55-57) */
+typedef struct mp_paged mp_paged_t;     /* paged K/V cache: what FlashInfer's paged cache is to models/attnserver.py:73-106 */
 typedef void* mp_stream_t;              /* hipStream_t */
 
 /* ---------------------------------------------------------------- library */
@@ -398,6 +402,57 @@ int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_hea
                         int64_t v_head_stride, const int32_t* cu_seqlens, int num_seqs, int64_t num_tokens,
                         int num_attention_heads, int num_key_value_heads, int head_dim, float scale, uint16_t* output,
                         float* lse, mp_stream_t stream);
+
+/* ---------------------------------------------------------------- paged cache
+ * Keys and values of many requests in pages that any request may own, and the attention of each request's new tokens over
+ * its pages: flashinfer.append_paged_kv_cache and BatchDecodeWithPagedKVCacheWrapper of models/attnserver.py:73-106,
+ * 239-259, for one new token or many.  (mp_attn_t holds max_length rows per request instead.)
+ *
+ * append, read and attention describe their rows alike, in device memory:
+ *   cu_seqlens int32 [num_seqs + 1]  request b's new rows in the packed tensors: cu_seqlens[b] .. cu_seqlens[b + 1] (n_b, may be 0)
+ *   page_table int32 [num_seqs, pages_per_seq]  position p of request b lies in page page_table[b][p / page_size]
+ *   kv_len     int32 [num_seqs]      positions of request b, the new rows included: new row i is position kv_len[b] - n_b + i
+ * Rows in front of the first and behind the last request, and rows at positions below 0 (kv_len[b] < n_b), are not
+ * touched; in attention the latter give 0 and -inf.  A page may belong to several requests; two rows
+ * appended to one place in one call leave either.
+ * A page id outside [0, num_pages) or a kv_len outside [0, pages_per_seq * page_size] accesses nothing outside the cache: the
+ * row is skipped (append, read), or the output unspecified (attention), and mp_paged_check reports it.
+ * Tensors are bf16, 16-byte aligned, read through token and head strides that are multiples of 8 elements (token strides below 2^23;
+ * dims contiguous), and written contiguously.  Device pointers only.  The handle holds the pages alone: calls that read may overlap;
+ * attention's scratch memory is the caller's. */
+int mp_paged_create(mp_paged_t** out);
+int mp_paged_destroy(mp_paged_t* h);
+/* head_dim 64 or 128; page_size a power of two up to 4096; kv_format MP_KV_BF16 or MP_KV_E4M3.  Pages start zeroed. */
+int mp_paged_alloc(mp_paged_t* h, int num_layers, int num_attention_heads, int num_key_value_heads, int head_dim,
+                   int64_t num_pages, int page_size, int kv_format);
+/* k, v [num_tokens, Hkv, D] into the pages.  MP_KV_E4M3: a row (one head's K or V of a token) is stored as e4m3(x 2^-e) and e,
+ * the least integer >= -126 with max |x| <= 448 * 2^e; codes round to nearest even, products with 2^e are exact (where the
+ * result is a normal bf16 number).  Infinities and NaN become NaN and do not count for the maximum. */
+int mp_paged_append(mp_paged_t* h, int layer_id, const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                    const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens, int num_seqs,
+                    int64_t num_tokens, const int32_t* page_table, int pages_per_seq, const int32_t* kv_len,
+                    mp_stream_t stream);
+/* The inverse: the same rows out of the pages, bf16 [num_tokens, Hkv, D] (MP_KV_E4M3: what the codes stand for). */
+int mp_paged_read(mp_paged_t* h, int layer_id, uint16_t* k, uint16_t* v, const int32_t* cu_seqlens, int num_seqs,
+                  int64_t num_tokens, const int32_t* page_table, int pages_per_seq, const int32_t* kv_len,
+                  mp_stream_t stream);
+/* New row i of request b attends to the request's positions 0 .. kv_len[b] - n_b + i as the cache holds them.
+ * q [num_tokens, H, D]; output bf16 [num_tokens, H, D]; lse f32 [num_tokens, H] (base 2, may be NULL); scale > 0.
+ * workspace: at least mp_paged_workspace(...) bytes, 16-byte aligned, not shared with a call that may run at the same time
+ * (may be NULL where that is 0); its contents need no preparation.  The keys of a row are split over workgroups when the
+ * rows are few, and joined in a fixed order: results do not vary from run to run. */
+int mp_paged_workspace(mp_paged_t* h, int num_seqs, int64_t num_tokens, int pages_per_seq, int64_t* bytes);
+int mp_paged_attention(mp_paged_t* h, int layer_id, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                       const int32_t* cu_seqlens, int num_seqs, int64_t num_tokens, const int32_t* page_table,
+                       int pages_per_seq, const int32_t* kv_len, float scale, uint16_t* output, float* lse, void* workspace,
+                       int64_t workspace_bytes, mp_stream_t stream);
+/* Waits for `stream`; MP_ERR_DATA if a call since the last check met a bad page id or length. */
+int mp_paged_check(mp_paged_t* h, mp_stream_t stream);
+/* Device views: pages [num_pages, Hkv, page_size, 2 (K, V), D] of bf16 or e4m3; scales u8 [num_pages, Hkv, page_size, 2]
+ * holding e + 127 (NULL for MP_KV_BF16). */
+int mp_paged_get_pages(mp_paged_t* h, int layer_id, void** pages_dev, void** scales_dev);
+/* HBM per layer, bytes: [0] rows, [1] scales. */
+int mp_paged_get_footprint(mp_paged_t* h, int64_t* bytes2);
 
 /* ---------------------------------------------------------------- LSE merge
  * Replaces flashinfer.merge_state as called at models/attnserver.py:308 (base-2 LSEs):

@@ -7,6 +7,7 @@ of the reference's operator API over it:
     from magicpig_amd import LSH, SparseAttentionServer        # library/lsh, library/sparse_attention
     from magicpig_amd import SimHash, LSHSparseAttnServer      # models/attnserver.py hot path
     from magicpig_amd import prompt_attention                  # causal attention over whole prompts, packed
+    from magicpig_amd import PagedKVCache                      # paged cache (bf16, e4m3) and attention over it
 
 Drop-in module names `lsh` and `sparse_attention_cpu` live in magicpig_amd/dropin (put that
 directory on PYTHONPATH, or call magicpig_amd.install_dropin()).
@@ -15,6 +16,7 @@ from .lsh import LSH  # noqa: F401
 from .simhash import SimHash  # noqa: F401
 from .sparse_attention import SparseAttentionServer  # noqa: F401
 from .attnserver import LSHSparseAttnServer  # noqa: F401
+from .paged_cache import PagedKVCache  # noqa: F401
 from .prompt_attention import prompt_attention  # noqa: F401
 from ._lib import MagicPigError  # noqa: F401
 

@@ -19,6 +19,7 @@ MP_OK = 0
 ERR_UNSUPPORTED = 5
 MEM_HOST, MEM_DEVICE = 0, 1
 DTYPE_BF16, DTYPE_F32 = 0, 1
+KV_FORMATS = {"bf16": 0, "e4m3": 1}
 DECODE_NO_BYPRODUCTS = 1      # mp_decode_*_ex flag (include/magicpig_hip.h)
 
 _ERR_NAMES = {1: "MP_ERR_INVALID", 2: "MP_ERR_STATE", 3: "MP_ERR_HIP", 4: "MP_ERR_NOMEM",
@@ -95,6 +96,16 @@ def lib() -> C.CDLL:
         "mp_decode_sparse_layer_ex": ([p, p, p, i32, p, p, p, p, C.c_uint, p], i32),
         "mp_decode_layer_window_ex": ([p, p, p, p, i32, p, p, p, p, p, C.c_uint, p], i32),
         "mp_prompt_attention": ([p, i64, i64, p, i64, i64, p, i64, i64, p, i32, i64, i32, i32, i32, C.c_float, p, p, p], i32),
+        "mp_paged_create": ([pp], i32),
+        "mp_paged_destroy": ([p], i32),
+        "mp_paged_alloc": ([p, i32, i32, i32, i32, i64, i32, i32], i32),
+        "mp_paged_append": ([p, i32, p, i64, i64, p, i64, i64, p, i32, i64, p, i32, p, p], i32),
+        "mp_paged_read": ([p, i32, p, p, p, i32, i64, p, i32, p, p], i32),
+        "mp_paged_workspace": ([p, i32, i64, i32, C.POINTER(i64)], i32),
+        "mp_paged_attention": ([p, i32, p, i64, i64, p, i32, i64, p, i32, p, C.c_float, p, p, p, i64, p], i32),
+        "mp_paged_check": ([p, p], i32),
+        "mp_paged_get_pages": ([p, i32, pp, pp], i32),
+        "mp_paged_get_footprint": ([p, C.POINTER(i64)], i32),
         "mp_merge_state": ([p, p, p, p, i32, i32, p, p, p], i32),
     }
     for name, (args, res) in sig.items():

@@ -18,12 +18,12 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 OBJDIR = os.path.join(LIBDIR, "obj")
 LIB = os.path.join(LIBDIR, "libmagicpig_hip.so")
-SOURCES = ["simhash.hip", "lsh.hip", "attention.hip", "prompt.hip", "capi.hip"]
+SOURCES = ["simhash.hip", "lsh.hip", "attention.hip", "prompt.hip", "paged.hip", "capi.hip"]
 ARCH = "gfx950"
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function"]
 # no packed f32 arithmetic (v_pk_*_f32) in these: some of its forms have returned wrong values on this part now and then
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCE_FLAGS = {"prompt.hip": NO_PACKED_F32}
+SOURCE_FLAGS = {"prompt.hip": NO_PACKED_F32, "paged.hip": NO_PACKED_F32}
 
 
 def _hipcc() -> str:

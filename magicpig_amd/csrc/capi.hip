@@ -1747,6 +1747,185 @@ int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_hea
     return MP_OK;
 }
 
+// =================================================================== paged cache
+
+int mp_paged_create(mp_paged_t** out) {
+    MP_REQUIRE(out != nullptr, MP_ERR_INVALID, "mp_paged_create: null out");
+    *out = new (std::nothrow) mp_paged();
+    MP_REQUIRE(*out != nullptr, MP_ERR_NOMEM, "mp_paged_create: out of host memory");
+    return MP_OK;
+}
+
+static void paged_free(mp_paged_t* h) {
+    for (int i = 0; i < h->layers; ++i) {
+        if (h->pool && h->pool[i]) (void)hipFree(h->pool[i]);
+        if (h->scale && h->scale[i]) (void)hipFree(h->scale[i]);
+    }
+    delete[] h->pool;
+    delete[] h->scale;
+    if (h->err) (void)hipFree(h->err);
+    h->pool = nullptr; h->scale = nullptr; h->err = nullptr;
+    h->allocated = false;
+}
+
+int mp_paged_destroy(mp_paged_t* h) {
+    MP_ON_DEVICE(h);
+    if (!h) return MP_OK;
+    paged_free(h);
+    delete h;
+    return MP_OK;
+}
+
+int mp_paged_alloc(mp_paged_t* h, int num_layers, int num_attention_heads, int num_key_value_heads, int head_dim,
+                   int64_t num_pages, int page_size, int kv_format) {
+    MP_REQUIRE(h, MP_ERR_INVALID, "mp_paged_alloc: null handle");
+    MP_REQUIRE(!h->allocated, MP_ERR_STATE, "mp_paged_alloc: already allocated");
+    MP_REQUIRE(head_dim == 64 || head_dim == 128, MP_ERR_UNSUPPORTED, "mp_paged_alloc: head_dim must be 64 or 128");
+    MP_REQUIRE(num_layers >= 1 && num_key_value_heads >= 1 && num_attention_heads >= num_key_value_heads &&
+                   num_attention_heads % num_key_value_heads == 0 && num_attention_heads <= 16384,
+               MP_ERR_INVALID, "mp_paged_alloc: bad head/layer counts");
+    MP_REQUIRE(page_size >= 1 && page_size <= 4096 && (page_size & (page_size - 1)) == 0, MP_ERR_INVALID,
+               "mp_paged_alloc: page_size must be a power of two up to 4096");
+    MP_REQUIRE(num_pages >= 1 && num_pages <= 0x7fffffff, MP_ERR_INVALID, "mp_paged_alloc: num_pages out of range");
+    MP_REQUIRE(kv_format == MP_KV_BF16 || kv_format == MP_KV_E4M3, MP_ERR_INVALID, "mp_paged_alloc: unknown kv_format");
+    MP_REQUIRE(num_pages <= (1ll << 48) / ((int64_t)num_key_value_heads * page_size * 4 * head_dim), MP_ERR_NOMEM,
+               "mp_paged_alloc: more pages than any memory holds");
+    h->device = current_device();
+    h->layers = num_layers; h->H = num_attention_heads; h->Hkv = num_key_value_heads; h->D = head_dim;
+    h->pages = num_pages; h->format = kv_format;
+    h->shift = __builtin_ctz((unsigned)page_size);
+    h->pool = new (std::nothrow) char*[num_layers]();
+    h->scale = new (std::nothrow) uint8_t*[num_layers]();
+    int rc = h->pool && h->scale ? MP_OK : fail(MP_ERR_NOMEM, "mp_paged_alloc: out of host memory");
+    for (int i = 0; i < num_layers && rc == MP_OK; ++i) {
+        rc = alloc_zero((void**)&h->pool[i], (size_t)(h->rows() * h->row_bytes()));
+        if (rc == MP_OK && kv_format == MP_KV_E4M3) rc = alloc_zero((void**)&h->scale[i], (size_t)(h->rows() * 2));
+    }
+    if (rc == MP_OK) rc = alloc_zero((void**)&h->err, 4);
+    if (rc == MP_OK && hipStreamSynchronize(nullptr) != hipSuccess)        // the zeros are there for calls on any stream
+        rc = fail(MP_ERR_HIP, "mp_paged_alloc: clearing the pages failed");
+    if (rc != MP_OK) { paged_free(h); return rc; }
+    hipDeviceProp_t prop;
+    if (hipGetDeviceProperties(&prop, h->device) == hipSuccess) h->cus = prop.multiProcessorCount;
+    h->allocated = true;
+    return MP_OK;
+}
+
+// what append, read and attention check alike
+static int paged_rows_check(mp_paged_t* h, int layer_id, const int32_t* cu, int num_seqs, int64_t num_tokens,
+                            const int32_t* table, int pages_per_seq, const int32_t* kv_len, const char* who) {
+    const std::string w(who);
+    MP_REQUIRE(h && h->allocated, MP_ERR_STATE, w + ": not allocated");
+    MP_REQUIRE(layer_id >= 0 && layer_id < h->layers, MP_ERR_INVALID, w + ": layer_id out of range");
+    MP_REQUIRE(num_seqs >= 1 && pages_per_seq >= 1 && num_tokens >= 0, MP_ERR_INVALID, w + ": bad request, page or token count");
+    MP_REQUIRE(num_tokens <= (1ll << 30) / (h->H / h->Hkv) && paged_copy_grid(num_tokens, h->Hkv, h->D) < (1ll << 31) - 1, MP_ERR_UNSUPPORTED,
+               w + ": more rows than one launch can number");
+    MP_REQUIRE(num_tokens == 0 || (cu && table && kv_len), MP_ERR_INVALID, w + ": null argument");
+    return MP_OK;
+}
+
+int mp_paged_append(mp_paged_t* h, int layer_id, const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                    const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens, int num_seqs,
+                    int64_t num_tokens, const int32_t* page_table, int pages_per_seq, const int32_t* kv_len,
+                    mp_stream_t stream) {
+    MP_ON_DEVICE(h);
+    if (int rc = paged_rows_check(h, layer_id, cu_seqlens, num_seqs, num_tokens, page_table, pages_per_seq, kv_len, "mp_paged_append"))
+        return rc;
+    if (num_tokens == 0) return MP_OK;
+    MP_REQUIRE(k && v, MP_ERR_INVALID, "mp_paged_append: null argument");
+    MP_REQUIRE(row_strides_ok(k_token_stride, k_head_stride) && row_strides_ok(v_token_stride, v_head_stride), MP_ERR_INVALID,
+               "mp_paged_append: strides must be multiples of 8 elements, token strides below 2^23");
+    MP_REQUIRE(aligned16(k) && aligned16(v), MP_ERR_INVALID, "mp_paged_append: k and v must be 16-byte aligned");
+    MP_HIP_CHECK(launch_paged_append(k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, cu_seqlens, num_seqs,
+                                     (int)num_tokens, page_table, pages_per_seq, kv_len, h->shift, (int)h->pages, h->Hkv, h->D,
+                                     h->format == MP_KV_E4M3, h->pool[layer_id], h->scale[layer_id], h->err, (hipStream_t)stream));
+    return MP_OK;
+}
+
+int mp_paged_read(mp_paged_t* h, int layer_id, uint16_t* k, uint16_t* v, const int32_t* cu_seqlens, int num_seqs,
+                  int64_t num_tokens, const int32_t* page_table, int pages_per_seq, const int32_t* kv_len,
+                  mp_stream_t stream) {
+    MP_ON_DEVICE(h);
+    if (int rc = paged_rows_check(h, layer_id, cu_seqlens, num_seqs, num_tokens, page_table, pages_per_seq, kv_len, "mp_paged_read"))
+        return rc;
+    if (num_tokens == 0) return MP_OK;
+    MP_REQUIRE(k && v, MP_ERR_INVALID, "mp_paged_read: null argument");
+    MP_REQUIRE(aligned16(k) && aligned16(v), MP_ERR_INVALID, "mp_paged_read: k and v must be 16-byte aligned");
+    MP_HIP_CHECK(launch_paged_read(k, v, cu_seqlens, num_seqs, (int)num_tokens, page_table, pages_per_seq, kv_len, h->shift,
+                                   (int)h->pages, h->Hkv, h->D, h->format == MP_KV_E4M3, h->pool[layer_id], h->scale[layer_id],
+                                   h->err, (hipStream_t)stream));
+    return MP_OK;
+}
+
+static int paged_parts_of(mp_paged_t* h, int num_seqs, int64_t num_tokens, int pages_per_seq) {
+    return paged_parts(num_tokens, num_seqs, h->H / h->Hkv, h->Hkv, (int64_t)pages_per_seq << h->shift, h->cus);
+}
+
+int mp_paged_workspace(mp_paged_t* h, int num_seqs, int64_t num_tokens, int pages_per_seq, int64_t* bytes) {
+    MP_REQUIRE(h && h->allocated, MP_ERR_STATE, "mp_paged_workspace: not allocated");
+    MP_REQUIRE(bytes && num_seqs >= 1 && pages_per_seq >= 1 && num_tokens >= 0, MP_ERR_INVALID, "mp_paged_workspace: bad argument");
+    *bytes = paged_workspace_bytes(num_tokens, h->H, h->D, paged_parts_of(h, num_seqs, num_tokens, pages_per_seq));
+    return MP_OK;
+}
+
+int mp_paged_attention(mp_paged_t* h, int layer_id, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                       const int32_t* cu_seqlens, int num_seqs, int64_t num_tokens, const int32_t* page_table,
+                       int pages_per_seq, const int32_t* kv_len, float scale, uint16_t* output, float* lse, void* workspace,
+                       int64_t workspace_bytes, mp_stream_t stream) {
+    MP_ON_DEVICE(h);
+    if (int rc = paged_rows_check(h, layer_id, cu_seqlens, num_seqs, num_tokens, page_table, pages_per_seq, kv_len, "mp_paged_attention"))
+        return rc;
+    MP_REQUIRE(attention_scale_ok(scale), MP_ERR_INVALID, "mp_paged_attention: scale must be finite and above 0");
+    if (num_tokens == 0) return MP_OK;
+    MP_REQUIRE(q && output, MP_ERR_INVALID, "mp_paged_attention: null argument");
+    MP_REQUIRE(row_strides_ok(q_token_stride, q_head_stride), MP_ERR_INVALID,
+               "mp_paged_attention: strides must be multiples of 8 elements, token strides below 2^23");
+    MP_REQUIRE(aligned16(q) && aligned16(output), MP_ERR_INVALID, "mp_paged_attention: q and output must be 16-byte aligned");
+    const int S = paged_parts_of(h, num_seqs, num_tokens, pages_per_seq);
+    MP_REQUIRE(paged_attention_grid(num_tokens, num_seqs, h->H / h->Hkv, h->Hkv, S) < (1ll << 31) - 1 &&
+                   paged_join_grid(num_tokens, h->H) < (1ll << 31) - 1,
+               MP_ERR_UNSUPPORTED, "mp_paged_attention: more rows than one launch can number");
+    const int64_t need = paged_workspace_bytes(num_tokens, h->H, h->D, S);
+    MP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), MP_ERR_INVALID,
+               "mp_paged_attention: workspace smaller than mp_paged_workspace says, or not 16-byte aligned");
+    MP_HIP_CHECK(launch_paged_attention(q, q_token_stride, q_head_stride, cu_seqlens, num_seqs, (int)num_tokens, page_table,
+                                        pages_per_seq, kv_len, h->shift, (int)h->pages, h->H, h->Hkv, h->D,
+                                        h->format == MP_KV_E4M3, h->pool[layer_id], h->scale[layer_id], h->err, scale * LOG2E,
+                                        S, output, lse, (char*)workspace, (hipStream_t)stream));
+    return MP_OK;
+}
+
+int mp_paged_check(mp_paged_t* h, mp_stream_t stream) {
+    MP_ON_DEVICE(h);
+    MP_REQUIRE(h && h->allocated, MP_ERR_STATE, "mp_paged_check: not allocated");
+    hipStream_t st = (hipStream_t)stream;
+    int flag = 0;
+    MP_HIP_CHECK(hipMemcpyAsync(&flag, h->err, 4, hipMemcpyDeviceToHost, st));
+    MP_HIP_CHECK(hipStreamSynchronize(st));
+    if (flag) {
+        MP_HIP_CHECK(hipMemsetAsync(h->err, 0, 4, st));
+        MP_HIP_CHECK(hipStreamSynchronize(st));
+        return fail(MP_ERR_DATA, flag & 1 ? "paged cache: a kv_len below 0 or beyond its page table"
+                                          : "paged cache: a page id outside the cache");
+    }
+    return MP_OK;
+}
+
+int mp_paged_get_pages(mp_paged_t* h, int layer_id, void** pages_dev, void** scales_dev) {
+    MP_REQUIRE(h && h->allocated, MP_ERR_STATE, "mp_paged_get_pages: not allocated");
+    MP_REQUIRE(layer_id >= 0 && layer_id < h->layers && pages_dev && scales_dev, MP_ERR_INVALID, "mp_paged_get_pages: bad argument");
+    *pages_dev = h->pool[layer_id];
+    *scales_dev = h->scale[layer_id];
+    return MP_OK;
+}
+
+int mp_paged_get_footprint(mp_paged_t* h, int64_t* bytes2) {
+    MP_REQUIRE(h && h->allocated && bytes2, MP_ERR_STATE, "mp_paged_get_footprint: not allocated");
+    bytes2[0] = h->rows() * h->row_bytes();
+    bytes2[1] = h->format == MP_KV_E4M3 ? h->rows() * 2 : 0;
+    return MP_OK;
+}
+
 // =================================================================== LSE merge
 
 int mp_merge_state(const uint16_t* va, const float* sa, const uint16_t* vb, const float* sb, int R,

@@ -140,6 +140,18 @@ struct mp_attn {
     int cus = 256;
 };
 
+struct mp_paged {
+    int device = -1;
+    int layers = 0, H = 0, Hkv = 0, D = 0, shift = 0, format = 0, cus = 256;
+    int64_t pages = 0;
+    bool allocated = false;
+    char** pool = nullptr;         // per layer, see paged.hip
+    uint8_t** scale = nullptr;     // per layer, null for MP_KV_BF16
+    int* err = nullptr;            // device: what the kernels met (1 = kv_len, 2 = page id)
+    int64_t rows() const { return pages * Hkv << shift; }
+    int64_t row_bytes() const { return 2 * (int64_t)D * (format == MP_KV_E4M3 ? 1 : 2); }
+};
+
 // the lsh handle whose last MP_MEM_HOST batch_retrieve is still described by its host_ret (nullptr: none); written
 // by that handle's calls, read by the attention entry.  Handles are not thread-safe (as the reference's objects);
 // the mutex only keeps a destroy on another thread from racing the lookup.

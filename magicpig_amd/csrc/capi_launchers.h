@@ -1,11 +1,11 @@
-// capi_launchers.h -- the kernels' host launchers (simhash.hip, lsh.hip, attention.hip, prompt.hip) as the C ABI's entry points call them
+// capi_launchers.h -- the kernels' host launchers (simhash.hip, lsh.hip, attention.hip, prompt.hip, paged.hip) as the C ABI's entry points call them
 // (one of the pieces capi.hip is made of: included there, once, in this order; not a header for other translation units)
 #pragma once
 
 namespace mp {
 
 
-// ---- kernels' host launchers (simhash.hip, lsh.hip, attention.hip, prompt.hip)
+// ---- kernels' host launchers (simhash.hip, lsh.hip, attention.hip, prompt.hip, paged.hip)
 int simhash_padded_cols(int K, int L);
 int simhash_supported(int D, int K);
 hipError_t launch_simhash_prepare(const uint16_t*, int, int, int, uint16_t*, uint16_t*, float*, hipStream_t);
@@ -71,6 +71,18 @@ int64_t prompt_grid(int64_t T, int B, int G, int Hkv);
 hipError_t launch_prompt_attention(const uint16_t*, int64_t, int64_t, const uint16_t*, int64_t, int64_t, const uint16_t*,
                                    int64_t, int64_t, const int32_t*, int, int, int, int, int, float, uint16_t*, float*,
                                    hipStream_t);
+int64_t paged_copy_grid(int64_t T, int Hkv, int D);
+int64_t paged_attention_grid(int64_t T, int B, int G, int Hkv, int S);
+int64_t paged_join_grid(int64_t T, int H);
+int paged_parts(int64_t T, int B, int G, int Hkv, int64_t capacity, int cus);
+int64_t paged_workspace_bytes(int64_t T, int H, int D, int S);
+hipError_t launch_paged_append(const uint16_t*, int64_t, int64_t, const uint16_t*, int64_t, int64_t, const int32_t*, int, int,
+                               const int32_t*, int, const int32_t*, int, int, int, int, bool, char*, uint8_t*, int*, hipStream_t);
+hipError_t launch_paged_read(uint16_t*, uint16_t*, const int32_t*, int, int, const int32_t*, int, const int32_t*, int, int, int,
+                             int, bool, char*, uint8_t*, int*, hipStream_t);
+hipError_t launch_paged_attention(const uint16_t*, int64_t, int64_t, const int32_t*, int, int, const int32_t*, int,
+                                  const int32_t*, int, int, int, int, int, bool, const char*, const uint8_t*, int*, float, int,
+                                  uint16_t*, float*, char*, hipStream_t);
 bool lsh_hash_only_supported(int L);
 hipError_t launch_attn_ticket_check(int*, int, int*, hipStream_t);
 hipError_t launch_relay(const void*, void*, size_t, hipStream_t);

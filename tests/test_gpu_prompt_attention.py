@@ -123,6 +123,18 @@ def test_empty_inputs():
     assert out.shape == (0, 8, 128) and lse.shape == (0, 8)
 
 
+@pytest.mark.gpu
+def test_refusals_of_shapes_and_devices():
+    q, k, v, cu = packed([4], 8, 2, 128)
+    for args, word in (((q, k[:, :, :64], v, cu), "k: expected shape"), ((q, k[:3], v, cu), "tokens"), ((q, k, v[:, :1], cu), "v: expected"),
+                       ((q, k, v, cu.cpu()), "cu_seqlens: on cpu"), ((q, k, v, cu[:1]), "cu_seqlens"),
+                       ((q[:, :, ::2], k[:, :, ::2], v[:, :, ::2], cu), "contiguous")):
+        with pytest.raises(ValueError, match=word):
+            mp.prompt_attention(*args)
+    with pytest.raises(TypeError, match="cu_seqlens"):
+        mp.prompt_attention(q, k, v, cu.long())
+
+
 # ---------------------------------------------------------------- refusals: nothing reaches the GPU
 GOOD = dict(q=1 << 20, qt=1024, qh=128, k=1 << 20, kt=256, kh=128, v=1 << 20, vt=256, vh=128, cu=1 << 20, seqs=2, tokens=10,
             H=8, Hkv=2, D=128, scale=0.1, out=1 << 20, lse=1 << 20, stream=None)
@@ -149,7 +161,5 @@ def test_refusals_of_the_python_entry():
         mp.prompt_attention(x, kv, kv, cu)
     with pytest.raises(TypeError, match="dtype"):
         mp.prompt_attention(x.float(), kv, kv, cu)
-    with pytest.raises(ValueError, match="shape"):
-        mp.prompt_attention(x.cuda() if torch.cuda.is_available() else x, kv[:, :, :64], kv, cu)
     with pytest.raises(ValueError, match="q:"):
         mp.prompt_attention(x[0], kv, kv, cu)
