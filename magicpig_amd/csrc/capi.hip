@@ -1857,14 +1857,10 @@ int mp_paged_read(mp_paged_t* h, int layer_id, uint16_t* k, uint16_t* v, const i
     return MP_OK;
 }
 
-static int paged_parts_of(mp_paged_t* h, int num_seqs, int64_t num_tokens, int pages_per_seq) {
-    return paged_parts(num_tokens, num_seqs, h->H / h->Hkv, h->Hkv, (int64_t)pages_per_seq << h->shift, h->cus);
-}
-
 int mp_paged_workspace(mp_paged_t* h, int num_seqs, int64_t num_tokens, int pages_per_seq, int64_t* bytes) {
     MP_REQUIRE(h && h->allocated, MP_ERR_STATE, "mp_paged_workspace: not allocated");
     MP_REQUIRE(bytes && num_seqs >= 1 && pages_per_seq >= 1 && num_tokens >= 0, MP_ERR_INVALID, "mp_paged_workspace: bad argument");
-    *bytes = paged_workspace_bytes(num_tokens, h->H, h->D, paged_parts_of(h, num_seqs, num_tokens, pages_per_seq));
+    *bytes = paged_workspace_bytes(num_tokens, num_seqs, h->H, h->Hkv, h->D, (int64_t)pages_per_seq << h->shift, h->cus);
     return MP_OK;
 }
 
@@ -1881,17 +1877,17 @@ int mp_paged_attention(mp_paged_t* h, int layer_id, const uint16_t* q, int64_t q
     MP_REQUIRE(row_strides_ok(q_token_stride, q_head_stride), MP_ERR_INVALID,
                "mp_paged_attention: strides must be multiples of 8 elements, token strides below 2^23");
     MP_REQUIRE(aligned16(q) && aligned16(output), MP_ERR_INVALID, "mp_paged_attention: q and output must be 16-byte aligned");
-    const int S = paged_parts_of(h, num_seqs, num_tokens, pages_per_seq);
-    MP_REQUIRE(paged_attention_grid(num_tokens, num_seqs, h->H / h->Hkv, h->Hkv, S) < (1ll << 31) - 1 &&
-                   paged_join_grid(num_tokens, h->H) < (1ll << 31) - 1,
+    const int64_t capacity = (int64_t)pages_per_seq << h->shift;
+    MP_REQUIRE(num_tokens * h->H < (1ll << 31) - 1 &&
+                   paged_attention_grid(num_tokens, num_seqs, h->H, h->Hkv, h->D, capacity, h->cus) < (1ll << 31) - 1,
                MP_ERR_UNSUPPORTED, "mp_paged_attention: more rows than one launch can number");
-    const int64_t need = paged_workspace_bytes(num_tokens, h->H, h->D, S);
+    const int64_t need = paged_workspace_bytes(num_tokens, num_seqs, h->H, h->Hkv, h->D, capacity, h->cus);
     MP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), MP_ERR_INVALID,
                "mp_paged_attention: workspace smaller than mp_paged_workspace says, or not 16-byte aligned");
     MP_HIP_CHECK(launch_paged_attention(q, q_token_stride, q_head_stride, cu_seqlens, num_seqs, (int)num_tokens, page_table,
                                         pages_per_seq, kv_len, h->shift, (int)h->pages, h->H, h->Hkv, h->D,
                                         h->format == MP_KV_E4M3, h->pool[layer_id], h->scale[layer_id], h->err, scale * LOG2E,
-                                        S, output, lse, (char*)workspace, (hipStream_t)stream));
+                                        h->cus, output, lse, (char*)workspace, (hipStream_t)stream));
     return MP_OK;
 }
 

@@ -72,10 +72,8 @@ hipError_t launch_prompt_attention(const uint16_t*, int64_t, int64_t, const uint
                                    int64_t, int64_t, const int32_t*, int, int, int, int, int, float, uint16_t*, float*,
                                    hipStream_t);
 int64_t paged_copy_grid(int64_t T, int Hkv, int D);
-int64_t paged_attention_grid(int64_t T, int B, int G, int Hkv, int S);
-int64_t paged_join_grid(int64_t T, int H);
-int paged_parts(int64_t T, int B, int G, int Hkv, int64_t capacity, int cus);
-int64_t paged_workspace_bytes(int64_t T, int H, int D, int S);
+int64_t paged_attention_grid(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus);
+int64_t paged_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus);
 hipError_t launch_paged_append(const uint16_t*, int64_t, int64_t, const uint16_t*, int64_t, int64_t, const int32_t*, int, int,
                                const int32_t*, int, const int32_t*, int, int, int, int, bool, char*, uint8_t*, int*, hipStream_t);
 hipError_t launch_paged_read(uint16_t*, uint16_t*, const int32_t*, int, int, const int32_t*, int, const int32_t*, int, int, int,

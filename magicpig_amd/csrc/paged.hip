@@ -130,43 +130,103 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(const CopyArgs a) {
 }
 
 // ---------------------------------------------------------------- attention over the pages
+// Work.  Request b has ceil(n_b G / BM) tiles of rows and ceil(kv_b / TOK) tiles of keys.  A workgroup gets one tile of rows
+// of one kv head and at most `per` tiles of keys; per is the mean of what `units` workgroups a kv head would get, found by every
+// workgroup from the lengths on the device (so a captured graph follows them), at least MIN_KEYS tokens: short requests are
+// one part, long ones are cut into parts of one size, whatever the mix.  Parts of a row are joined by a second kernel.
 struct PagedAttnArgs {
     PagedRows r;
     const uint16_t* q;
     int64_t q_st, q_sh;
     const char* pool;
     const uint8_t* scale;
-    int H, G, slots, S;              // S: parts the keys of a row tile may be cut into
+    int H, G, units;                 // units: 0 = never cut the keys
     float c;
     uint16_t* out;
     float* lse;
-    float* part_o;                   // [S][T * H][D], sums that are not normalised
-    float2* part_ml;                 // [S][T * H], their maxima and sums of weights
-    int* part_n;                     // [T * H], parts in use
+    float* part_o;                   // [workgroup][BM][D], sums that are not normalised
+    float2* part_ml;                 // [workgroup][BM], their maxima and sums of weights
+    int2* part_of;                   // [T * H]: the row's place among the part_o of its first part, number of parts
+    int grid;                        // workgroups
 };
 
-constexpr int MIN_TILES = 4;         // a part is at least this many tiles: below, joining costs more than it spreads
+constexpr int MIN_KEYS = 256;        // a part is at least this long: below, joining costs more than it spreads
 
-// A workgroup owns 128 rows of one (request, kv head) and one part of its keys; everything else is as in prompt.hip.  An
-// e4m3 tile passes through registers on its way to LDS: loaded while the tile before it is folded in, widened
-// (v_cvt_scalef32_pk_bf16_fp8: exact) behind it.
+struct PartOf {
+    int seq;                         // -1: none
+    int start, n, row0, kv;          // first row of q (token) and tokens of the request, first row of the tile, cached positions
+    int part, per;                   // which part, tiles of keys a part has
+};
+
+template <int BM, int TOK>
+__device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units, int unit) {
+    PartOf p;
+    p.seq = -1;
+    p.start = p.n = p.row0 = p.kv = p.part = 0;
+    auto first = [&](int i) { return min(max(r.cu[i], 0), r.T); };
+    auto row_tiles = [&](int i) { return (max(first(i + 1) - first(i), 0) * G + BM - 1) / BM; };
+    auto key_tiles = [&](int i) { return (int)(((int64_t)cached(r, i) + TOK - 1) / TOK); };
+    p.per = 0x7fffffff;
+    if (units > 0) {
+        float work = 0.f;            // (products of large counts; the quotient need not be exact)
+        for (int base = 0; base < r.B; base += WAVE) {
+            const int i = base + lane_id();
+            if (i < r.B) work += (float)row_tiles(i) * (float)key_tiles(i);
+        }
+        p.per = max((int)__builtin_ceilf(fminf(wave_sum(work) / (float)units, 1e9f)), MIN_KEYS / TOK);
+    }
+    int before = 0;
+    for (int base = 0; base < r.B; base += WAVE) {
+        const int i = base + lane_id();
+        const int rt = i < r.B ? row_tiles(i) : 0;
+        const int parts = rt > 0 ? max((key_tiles(i) + p.per - 1) / p.per, 1) : 0;
+        const int sum = before + wave_incl_scan(rt * parts);
+        const unsigned long long past = __ballot(sum > unit);
+        if (past) {
+            const int k = __ffsll(past) - 1;
+            const int np = __builtin_amdgcn_readlane(parts, k);
+            const int at = unit - (__builtin_amdgcn_readlane(sum, k) - __builtin_amdgcn_readlane(rt, k) * np);
+            p.seq = base + k;
+            p.start = first(p.seq);
+            p.n = first(p.seq + 1) - p.start;
+            p.kv = cached(r, p.seq);
+            p.row0 = at / np * BM;
+            p.part = at % np;
+            return p;
+        }
+        before = __builtin_amdgcn_readlane(sum, WAVE - 1);
+    }
+    return p;
+}
+
+// e4m3 pairs -> bf16 pairs times a power of two
+__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float s) {
+    u32x4 w;
+    w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));
+    w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true));
+    w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false));
+    w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
+    return w;
+}
+
+// Many rows: 128 of one (request, kv head) a workgroup, everything else as in prompt.hip.  An e4m3 tile passes through
+// registers on its way to LDS: loaded while the tile before it is folded in, widened behind it (exact).
 template <int D, bool E4M3>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttnArgs a) {
     constexpr int BM = 128, CPR = D / 8, KB = TILE_TOKENS * 2 * D;
     constexpr int PER_ROW = E4M3 ? CPR / 2 : CPR;                     // 16-byte pieces of a cached row
     constexpr int PASSES = TILE_TOKENS * PER_ROW / 256;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][KB];
-    const int head = blockIdx.x % a.r.Hkv, split = (int)(blockIdx.x / a.r.Hkv) % a.S;
-    const TileOf t = find_tile<BM>(a.r.cu, a.r.B, a.r.T, a.G, a.slots - 1 - (int)(blockIdx.x / a.r.Hkv) / a.S);
+    const int head = blockIdx.x % a.r.Hkv;
+    const PartOf t = find_part<BM, TILE_TOKENS>(a.r, a.G, a.units, (int)(blockIdx.x / a.r.Hkv));
     if (t.seq < 0) return;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
-    const int rows = t.n * a.G, old = cached(a.r, t.seq) - t.n;       // old: positions in front of the new tokens
+    const int rows = t.n * a.G, old = t.kv - t.n;                     // old: positions in front of the new tokens
     const int lim_lo = old + t.row0 / a.G, lim_hi = old + min(t.row0 + BM - 1, rows - 1) / a.G;
     const int all = lim_hi < 0 ? 0 : lim_hi / TILE_TOKENS + 1;
-    const int per = max((all + a.S - 1) / a.S, MIN_TILES);
-    const int used = max((all + per - 1) / per, 1);
-    if (split >= used) return;
-    const int begin = split * per, end = min(all, begin + per);
+    const int used = all > t.per ? (all + t.per - 1) / t.per : 1;
+    if (t.part >= used) return;
+    const int begin = t.part * min(t.per, all), end = min(all, begin + min(t.per, all));
 
     const int wrow = t.row0 + 32 * w;
     const int row = min(wrow + (l & 31), rows - 1);
@@ -216,17 +276,8 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttn
             const float ks = __uint_as_float((sr[i] & 255u) << 23), vs = __uint_as_float((sr[i] >> 8) << 23);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                u32x4 kw, vw;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const uint32_t kc = kr[i][2 * e + x], vc = vr[i][2 * e + x];
-                    kw[2 * x] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kc, ks, false));
-                    kw[2 * x + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kc, ks, true));
-                    vw[2 * x] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vc, vs, false));
-                    vw[2 * x + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(vc, vs, true));
-                }
-                *reinterpret_cast<u32x4*>(kt + (((2 * p + e) ^ key_swizzle<D>(r)) << 4)) = kw;
-                *reinterpret_cast<u32x4*>(kt + KB + (((2 * p + e) ^ value_swizzle<D>(r)) << 4)) = vw;
+                *reinterpret_cast<u32x4*>(kt + (((2 * p + e) ^ key_swizzle<D>(r)) << 4)) = widen8(kr[i][2 * e], kr[i][2 * e + 1], ks);
+                *reinterpret_cast<u32x4*>(kt + KB + (((2 * p + e) ^ value_swizzle<D>(r)) << 4)) = widen8(vr[i][2 * e], vr[i][2 * e + 1], vs);
             }
         }
     };
@@ -252,13 +303,14 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttn
         next([&](const char* kt, const char* vt) { if (j < seen) fold_tile<D, 2, true>(st, kt, vt, a.c, lim - j * TILE_TOKENS); });
 
     if (wrow + (l & 31) >= rows) return;
-    const int64_t orow = (int64_t)(t.start + tok) * a.H + h, R = (int64_t)a.r.T * a.H;
-    if (split == 0 && a.S > 1 && l < 32) a.part_n[orow] = used;
+    const int64_t orow = (int64_t)(t.start + tok) * a.H + h;
+    if (a.units > 0 && t.part == 0 && l < 32) a.part_of[orow] = make_int2((int)blockIdx.x * BM + 32 * w + l, used);
     if (used == 1) {
         store_rows<D>(st, a.out + orow * D, a.lse ? a.lse + orow : nullptr);
         return;
     }
-    float* po = a.part_o + (split * R + orow) * D;
+    const int64_t prow = (int64_t)blockIdx.x * BM + 32 * w + (l & 31);
+    float* po = a.part_o + prow * D;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -266,41 +318,201 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttn
             *reinterpret_cast<f32x4*>(po + 32 * i + 8 * g + 4 * (l >> 5)) =
                 f32x4{st.o[i][4 * g], st.o[i][4 * g + 1], st.o[i][4 * g + 2], st.o[i][4 * g + 3]};
     const float sum = halves_sum(st.l);
-    if (l < 32) a.part_ml[split * R + orow] = make_float2(st.m, sum);
+    if (l < 32) a.part_ml[prow] = make_float2(st.m, sum);
 }
 
-// Parts of a row joined in their order: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, one wave a row.
-template <int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
-    const int64_t R = (int64_t)a.r.T * a.H, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= R) return;
-    const int tok = (int)(row / a.H), l = lane_id();
-    if (tok < a.r.cu[0] || tok >= a.r.cu[a.r.B]) return;              // (part_n of such a row was never written)
-    const int n = min(a.part_n[row], a.S);
-    if (n <= 1) return;
-    float m = NEG_INF;
-    for (int s = l; s < n; s += WAVE) m = fmaxf(m, a.part_ml[s * R + row].x);
-    m = wave_max(m);
+// Few rows (a decode step, drafted tokens): one tile of 32 rows a workgroup, and the keys are what is shared out -- tiles
+// of 32 tokens in turn over the four waves, each with its own running softmax over its own block of LDS (no barrier until
+// the waves' results are joined at the end).  A tile passes through registers: its loads (16 KB a wave in bf16, 8 KB in
+// e4m3, eight waves a CU) are in flight while the tile before it is folded in.
+template <int D, bool E4M3>
+__global__ __launch_bounds__(256, 2) void paged_step_kernel(const PagedAttnArgs a) {
+    constexpr int BM = 32, TOK = 32, KB = TOK * 2 * D, NC = D / 4;     // NC: 16-byte chunks of an f32 row
+    constexpr int PER_ROW = E4M3 ? D / 16 : D / 8;
+    constexpr int PASSES = TOK * PER_ROW / 64;
+    __shared__ __attribute__((aligned(1024))) char lds[4][2 * KB];     // a wave's K and V tile; at the end its 32 rows of sums
+    __shared__ float2 ml[4][BM];
+    const int head = blockIdx.x % a.r.Hkv;
+    const PartOf t = find_part<BM, TOK>(a.r, a.G, a.units, (int)(blockIdx.x / a.r.Hkv));
+    if (t.seq < 0) return;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
+    const int rows = t.n * a.G, old = t.kv - t.n;
+    const int lim_lo = old + t.row0 / a.G, lim_hi = old + min(t.row0 + BM - 1, rows - 1) / a.G;
+    const int all = lim_hi < 0 ? 0 : lim_hi / TOK + 1;
+    const int used = all > t.per ? (all + t.per - 1) / t.per : 1;
+    if (t.part >= used) return;
+    const int begin = t.part * min(t.per, all), end = min(all, begin + min(t.per, all));
+    const int whole = min(lim_lo < 0 ? 0 : (lim_lo + 1) / TOK, end);
+
+    RowState<D> st;
+    const int row = min(t.row0 + (l & 31), rows - 1), tok = row / a.G, lim = old + tok;
+    load_rows<D>(st, a.q + (int64_t)(t.start + tok) * a.q_st + (int64_t)(head * a.G + row % a.G) * a.q_sh);
+
+    const int32_t* table = a.r.table + (int64_t)t.seq * a.r.P;
+    const int slot_mask = (1 << a.r.shift) - 1;
+    char *kt = lds[w], *vt = lds[w] + KB;
+    // lane l looks up the cache row of token l % 32 of a tile (positions behind the last visible one: that one again,
+    // masked); the lanes that load a row get it from there.  (A row number fits 32 bits: 2^32 rows are more than any HBM.)
+    int page = 0;
+    u32x4 kr[PASSES], vr[PASSES];
+    uint32_t sr[PASSES];
+    auto position = [&](int tile) { return min(tile * TOK + (l & 31), lim_hi); };
+    auto fetch_pages = [&](int tile) { page = table[position(tile) >> a.r.shift]; };
+    auto load = [&](int tile) {
+        const int pg = max(page_ok(a.r, page), 0);
+        int l = lane_id();
+        asm volatile("" : "+v"(l));          // (the few things below that depend on it are not worth registers of their own)
+        const uint32_t at = (((uint32_t)pg * (uint32_t)a.r.Hkv + (uint32_t)head) << a.r.shift) | (uint32_t)(position(tile) & slot_mask);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int r = (i * 64 + l) / PER_ROW, p = (i * 64 + l) % PER_ROW;
+            const uint64_t x = (uint32_t)__builtin_amdgcn_ds_bpermute(r * 4, (int)at);
+            const char* src = a.pool + x * (E4M3 ? 2 * D : 4 * D) + p * 16;
+            kr[i] = *reinterpret_cast<const u32x4*>(src);
+            vr[i] = *reinterpret_cast<const u32x4*>(src + (E4M3 ? D : 2 * D));
+            if (E4M3) sr[i] = *reinterpret_cast<const uint16_t*>(a.scale + x * 2);
+        }
+    };
+    // (within a wave LDS works in order: what the lanes wrote is there for the reads behind it, and the tile's last reads are
+    // in front of the next writes; the fences keep the compiler to that order)
+    auto store = [&]() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int r = (i * 64 + l) / PER_ROW, p = (i * 64 + l) % PER_ROW;
+            char *kd = kt + r * 2 * D, *vd = vt + r * 2 * D;
+            if (!E4M3) {
+                *reinterpret_cast<u32x4*>(kd + ((p ^ key_swizzle<D>(r)) << 4)) = kr[i];
+                *reinterpret_cast<u32x4*>(vd + ((p ^ value_swizzle<D>(r)) << 4)) = vr[i];
+            } else {
+                const float ks = __uint_as_float((sr[i] & 255u) << 23), vs = __uint_as_float((sr[i] >> 8) << 23);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    *reinterpret_cast<u32x4*>(kd + (((2 * p + e) ^ key_swizzle<D>(r)) << 4)) = widen8(kr[i][2 * e], kr[i][2 * e + 1], ks);
+                    *reinterpret_cast<u32x4*>(vd + (((2 * p + e) ^ value_swizzle<D>(r)) << 4)) = widen8(vr[i][2 * e], vr[i][2 * e + 1], vs);
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    int j = begin + w;
+    if (j < end) {
+        fetch_pages(j);
+        load(j);
+        if (j + 4 < end) fetch_pages(j + 4);
+    }
+    auto ahead = [&] {
+        if (j + 4 < end) {
+            load(j + 4);
+            if (j + 8 < end) fetch_pages(j + 8);
+        }
+    };
+    for (; j < whole; j += 4) {
+        store();
+        __builtin_amdgcn_sched_barrier(0);           // the next tile's loads take the registers just stored
+        ahead();
+        fold_tile<D, 1, false>(st, kt, vt, a.c, 0);
+    }
+    for (; j < end; j += 4) {            // the last tile or two: nothing to load beside it, or little
+        store();
+        fold_tile<D, 1, true>(st, kt, vt, a.c, lim - j * TOK);
+        ahead();
+    }
+
+    // the four waves' sums, f32, row after row with chunks permuted (the rows of a column lie in one bank otherwise)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const float sum = halves_sum(st.l);
+    if (l < 32) ml[w][l] = make_float2(st.m, sum);
+    f32x4* mine = reinterpret_cast<f32x4*>(lds[w]) + (l & 31) * NC;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            mine[(8 * i + 2 * g + (l >> 5)) ^ (l & (NC - 1) & 31)] =
+                f32x4{st.o[i][4 * g], st.o[i][4 * g + 1], st.o[i][4 * g + 2], st.o[i][4 * g + 3]};
+    __syncthreads();
+    const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (NC / 8), grow = t.row0 + r;     // 8 threads a row
+    if (grow >= rows) return;
+    float2 x[4];
+    float m = NEG_INF, wt[4], total = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        x[k] = ml[k][r];
+        m = fmaxf(m, x[k].x);
+    }
     const float off = m == NEG_INF ? 0.f : m;
-    float sum = 0.f, o[D / 64];
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
-    for (int s0 = 0; s0 < n; s0 += WAVE) {
-        const float2 ml = s0 + l < n ? a.part_ml[(s0 + l) * R + row] : make_float2(NEG_INF, 0.f);
-        const float w = __builtin_amdgcn_exp2f(ml.x - off);
-        sum += wave_sum(w * ml.y);
-        const int k = min(n - s0, WAVE);
-        for (int s = 0; s < k; ++s) {
-            const float ws = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s));
-            const float* po = a.part_o + ((s0 + s) * R + row) * D + l * (D / 64);
+    for (int k = 0; k < 4; ++k) {
+        wt[k] = __builtin_amdgcn_exp2f(x[k].x - off);
+        total += wt[k] * x[k].y;
+    }
+    const int64_t orow = (int64_t)(t.start + grow / a.G) * a.H + head * a.G + grow % a.G;
+    const int64_t prow = (int64_t)blockIdx.x * BM + r;
+    const float inv = used > 1 ? 1.f : total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) o[i] += ws * po[i];
+    for (int c = 0; c < NC / 8; ++c) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const f32x4 y = reinterpret_cast<const f32x4*>(lds[k])[r * NC + ((c0 + c) ^ (r & (NC - 1) & 31))];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += wt[k] * y[e];
+        }
+        if (used > 1) {
+            *reinterpret_cast<f32x4*>(a.part_o + prow * D + 4 * (c0 + c)) = o;
+        } else {
+            u32x2 b;
+            b[0] = pack_bf16(o[0] * inv, o[1] * inv);
+            b[1] = pack_bf16(o[2] * inv, o[3] * inv);
+            *reinterpret_cast<u32x2*>(a.out + orow * D + 4 * (c0 + c)) = b;
         }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (D == 128) *reinterpret_cast<uint32_t*>(a.out + row * D + 2 * l) = pack_bf16(o[0] * inv, o[D / 64 - 1] * inv);
-    else a.out[row * D + l] = (uint16_t)(pack_bf16(o[0] * inv, 0.f) & 0xffffu);
-    if (a.lse != nullptr && l == 0) a.lse[row] = log_sum(m, sum);
+    if (c0 != 0) return;
+    if (a.units > 0 && t.part == 0) a.part_of[orow] = make_int2((int)blockIdx.x * BM + r, used);
+    if (used > 1) a.part_ml[prow] = make_float2(m, total);
+    else if (a.lse != nullptr) a.lse[orow] = log_sum(m, total);
+}
+
+// Parts of a row joined: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, in an order that does not depend on when they
+// were ready.  A workgroup a row, its waves take the parts in turn.
+template <int D, int BM>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
+    constexpr int W = D / 64;
+    __shared__ float so[4][D], sl[4];
+    const int64_t row = blockIdx.x;
+    const int tok = (int)(row / a.H), l = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (tok < a.r.cu[0] || tok >= a.r.cu[a.r.B]) return;              // (part_of of such a row was never written)
+    const int2 of = a.part_of[row];
+    const int n = of.y;
+    const int64_t at = of.x, step = (int64_t)a.r.Hkv * BM;            // the parts of a row are neighbours among its head's workgroups
+    if (n <= 1 || at < 0 || at + (n - 1) * step >= (int64_t)a.grid * BM) return;     // (offsets that are none could leave anything)
+    float m = NEG_INF;
+    for (int s = l; s < n; s += WAVE) m = fmaxf(m, a.part_ml[at + s * step].x);
+    m = wave_max(m);
+    const float off = m == NEG_INF ? 0.f : m;
+    float sum = 0.f, o[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) o[i] = 0.f;
+#pragma unroll 4
+    for (int s = w; s < n; s += 4) {
+        const float2 x = a.part_ml[at + s * step];
+        const float* po = a.part_o + (at + s * step) * D + l * W;
+        const float wt = __builtin_amdgcn_exp2f(x.x - off);
+        sum += wt * x.y;
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] += wt * po[i];
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) so[w][l * W + i] = o[i];
+    if (l == 0) sl[w] = sum;
+    __syncthreads();
+    if (threadIdx.x >= D / 2) return;
+    const float total = (sl[0] + sl[1]) + (sl[2] + sl[3]), inv = total == 0.f ? 0.f : 1.f / total;
+    const int d = 2 * threadIdx.x;
+    const float x = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
+    const float y = (so[0][d + 1] + so[1][d + 1]) + (so[2][d + 1] + so[3][d + 1]);
+    *reinterpret_cast<uint32_t*>(a.out + row * D + d) = pack_bf16(x * inv, y * inv);
+    if (a.lse != nullptr && threadIdx.x == 0) a.lse[row] = log_sum(m, total);
 }
 
 // ---------------------------------------------------------------- host
@@ -346,45 +558,65 @@ hipError_t launch_paged_read(uint16_t* k, uint16_t* v, const int32_t* cu, int B,
     return hipGetLastError();
 }
 
-static int64_t paged_slots(int64_t T, int B, int G) { return T * G / 128 + B; }
-int64_t paged_attention_grid(int64_t T, int B, int G, int Hkv, int S) { return paged_slots(T, B, G) * Hkv * S; }
-int64_t paged_join_grid(int64_t T, int H) { return (T * H + 3) / 4; }
-
-// Parts: enough that the row tiles fill the chip (two workgroups a CU), never finer than MIN_TILES tiles of the longest
-// possible key list.
-int paged_parts(int64_t T, int B, int G, int Hkv, int64_t capacity, int cus) {
-    const int64_t tiles = (T * G / 128 + (T < B ? T : B)) * Hkv;
-    const int64_t most = (capacity + MIN_TILES * TILE_TOKENS - 1) / (MIN_TILES * TILE_TOKENS);
-    int64_t S = 2 * (int64_t)cus / (tiles > 0 ? tiles : 1);
-    if (S > most) S = most;
-    return S < 1 ? 1 : (int)S;
+// How attention cuts a call's work, from what the host knows.
+struct PagedPlan {
+    bool step;           // 32 rows a workgroup (few rows a request) instead of 128
+    int units;           // workgroups a kv head that the keys are cut for, 0 = not cut
+    int64_t grid;        // workgroups, at most
+    int64_t bytes;       // workspace
+};
+PagedPlan paged_plan(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus) {
+    const int64_t G = H / Hkv, live = T < B ? T : B;
+    PagedPlan p;
+    // by the mean rows of a request and kv head: up to one tile of 32 the keys are read once either way
+    p.step = T * G <= 32 * live;
+    const int BM = p.step ? 32 : 128;
+    const int64_t tiles = T * G / BM + live, target = 2 * (int64_t)cus;           // two workgroups a CU
+    // rows alone that give every CU eight workgroups are not cut further; neither is what fits one part
+    p.units = tiles * Hkv >= 4 * target || capacity <= MIN_KEYS ? 0 : (int)((target + Hkv - 1) / Hkv);
+    p.grid = (tiles + p.units + (p.units > 0)) * Hkv;
+    p.bytes = p.units > 0 ? p.grid * BM * ((int64_t)D * 4 + 8) + T * H * 8 : 0;
+    return p;
 }
-int64_t paged_workspace_bytes(int64_t T, int H, int D, int S) {
-    return S > 1 ? S * T * H * ((int64_t)D * 4 + 8) + T * H * 4 : 0;
+
+template <int D, bool E4M3>
+static void paged_attention(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
+    const dim3 grid((unsigned)p.grid), join((unsigned)(a.r.T * a.H));
+    if (p.step) {
+        paged_step_kernel<D, E4M3><<<grid, 256, 0, st>>>(a);
+        if (p.units > 0) paged_join_kernel<D, 32><<<join, 256, 0, st>>>(a);
+    } else {
+        paged_attention_kernel<D, E4M3><<<grid, 256, 0, st>>>(a);
+        if (p.units > 0) paged_join_kernel<D, 128><<<join, 256, 0, st>>>(a);
+    }
+}
+
+int64_t paged_attention_grid(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus) {
+    return paged_plan(T, B, H, Hkv, D, capacity, cus).grid;
+}
+int64_t paged_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus) {
+    return paged_plan(T, B, H, Hkv, D, capacity, cus).bytes;
 }
 
 hipError_t launch_paged_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, const int32_t* cu, int B, int T,
                                   const int32_t* table, int P, const int32_t* kv_len, int shift, int num_pages, int H,
-                                  int Hkv, int D, bool e4m3, const char* pool, const uint8_t* scale, int* err, float c, int S,
+                                  int Hkv, int D, bool e4m3, const char* pool, const uint8_t* scale, int* err, float c, int cus,
                                   uint16_t* out, float* lse, char* ws, hipStream_t st) {
-    const int G = H / Hkv;
-    const int64_t R = (int64_t)T * H;
-    PagedAttnArgs a{paged_rows(cu, B, T, table, P, kv_len, shift, num_pages, Hkv, err), q, q_st, q_sh, pool, scale, H, G,
-                    (int)paged_slots(T, B, G), S, c, out, lse, nullptr, nullptr, nullptr};
-    if (S > 1) {
+    const PagedPlan p = paged_plan(T, B, H, Hkv, D, (int64_t)P << shift, cus);
+    PagedAttnArgs a{paged_rows(cu, B, T, table, P, kv_len, shift, num_pages, Hkv, err), q, q_st, q_sh, pool, scale, H, H / Hkv,
+                    p.units, c, out, lse, nullptr, nullptr, nullptr, (int)p.grid};
+    if (p.units > 0) {
+        const int64_t rows = p.grid * (p.step ? 32 : 128);
         a.part_o = reinterpret_cast<float*>(ws);
-        a.part_ml = reinterpret_cast<float2*>(ws + S * R * D * 4);
-        a.part_n = reinterpret_cast<int*>(ws + S * R * (D * 4 + 8));
+        a.part_ml = reinterpret_cast<float2*>(ws + rows * D * 4);
+        a.part_of = reinterpret_cast<int2*>(ws + rows * (D * 4 + 8));
     }
-    const dim3 grid((unsigned)paged_attention_grid(T, B, G, Hkv, S)), join((unsigned)paged_join_grid(T, H));
     if (D == 128) {
-        if (e4m3) paged_attention_kernel<128, true><<<grid, 256, 0, st>>>(a);
-        else paged_attention_kernel<128, false><<<grid, 256, 0, st>>>(a);
-        if (S > 1) paged_join_kernel<128><<<join, 256, 0, st>>>(a);
+        if (e4m3) paged_attention<128, true>(a, p, st);
+        else paged_attention<128, false>(a, p, st);
     } else {
-        if (e4m3) paged_attention_kernel<64, true><<<grid, 256, 0, st>>>(a);
-        else paged_attention_kernel<64, false><<<grid, 256, 0, st>>>(a);
-        if (S > 1) paged_join_kernel<64><<<join, 256, 0, st>>>(a);
+        if (e4m3) paged_attention<64, true>(a, p, st);
+        else paged_attention<64, false>(a, p, st);
     }
     return hipGetLastError();
 }
