@@ -167,6 +167,11 @@ def current_stream(ref: torch.Tensor | None = None, device: int | None = None) -
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def stream_on(index: int):
+    """hipStream_t of torch's current stream on GPU `index`, for callers that hold a tensor or handle of it."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def current_device() -> int:
     """Index of the current GPU (0 when there is none: the C ABI then fails with MP_ERR_HIP)."""
     return torch.cuda.current_device() if torch.cuda.is_available() else 0

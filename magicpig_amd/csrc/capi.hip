@@ -1788,7 +1788,8 @@ int mp_paged_alloc(mp_paged_t* h, int num_layers, int num_attention_heads, int n
                "mp_paged_alloc: page_size must be a power of two up to 4096");
     MP_REQUIRE(num_pages >= 1 && num_pages <= 0x7fffffff, MP_ERR_INVALID, "mp_paged_alloc: num_pages out of range");
     MP_REQUIRE(kv_format == MP_KV_BF16 || kv_format == MP_KV_E4M3, MP_ERR_INVALID, "mp_paged_alloc: unknown kv_format");
-    MP_REQUIRE(num_pages <= (1ll << 48) / ((int64_t)num_key_value_heads * page_size * 4 * head_dim), MP_ERR_NOMEM,
+    // (the kernels number the rows in 32 bits: at 128 bytes or more a row that is 512 GB)
+    MP_REQUIRE(num_pages < (1ll << 32) / ((int64_t)num_key_value_heads * page_size), MP_ERR_NOMEM,
                "mp_paged_alloc: more pages than any memory holds");
     h->device = current_device();
     h->layers = num_layers; h->H = num_attention_heads; h->Hkv = num_key_value_heads; h->D = head_dim;
@@ -1818,8 +1819,7 @@ static int paged_rows_check(mp_paged_t* h, int layer_id, const int32_t* cu, int 
     MP_REQUIRE(h && h->allocated, MP_ERR_STATE, w + ": not allocated");
     MP_REQUIRE(layer_id >= 0 && layer_id < h->layers, MP_ERR_INVALID, w + ": layer_id out of range");
     MP_REQUIRE(num_seqs >= 1 && pages_per_seq >= 1 && num_tokens >= 0, MP_ERR_INVALID, w + ": bad request, page or token count");
-    MP_REQUIRE(num_tokens <= (1ll << 30) / (h->H / h->Hkv) && paged_copy_grid(num_tokens, h->Hkv, h->D) < (1ll << 31) - 1, MP_ERR_UNSUPPORTED,
-               w + ": more rows than one launch can number");
+    MP_REQUIRE(num_tokens <= (1ll << 30) / (h->H / h->Hkv), MP_ERR_UNSUPPORTED, w + ": more rows than one launch can number");
     MP_REQUIRE(num_tokens == 0 || (cu && table && kv_len), MP_ERR_INVALID, w + ": null argument");
     return MP_OK;
 }

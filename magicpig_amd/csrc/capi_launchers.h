@@ -71,7 +71,6 @@ int64_t prompt_grid(int64_t T, int B, int G, int Hkv);
 hipError_t launch_prompt_attention(const uint16_t*, int64_t, int64_t, const uint16_t*, int64_t, int64_t, const uint16_t*,
                                    int64_t, int64_t, const int32_t*, int, int, int, int, int, float, uint16_t*, float*,
                                    hipStream_t);
-int64_t paged_copy_grid(int64_t T, int Hkv, int D);
 int64_t paged_attention_grid(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus);
 int64_t paged_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus);
 hipError_t launch_paged_append(const uint16_t*, int64_t, int64_t, const uint16_t*, int64_t, int64_t, const int32_t*, int, int,

@@ -23,9 +23,9 @@ struct PagedRows {
     int* err;
 };
 
-// cache length of request b, inside what its table can hold
-__device__ __forceinline__ int cached(const PagedRows& r, int b) {
-    const int want = r.kv_len[b], have = (int)min((int64_t)r.P << r.shift, (int64_t)0x7fffffff);
+// a request's cache length, inside what its table can hold
+__device__ __forceinline__ int cached(const PagedRows& r, int want) {
+    const int have = (int)min((int64_t)r.P << r.shift, (int64_t)0x7fffffff);
     if (want < 0 || want > have) {
         atomicOr(r.err, 1);
         return want < 0 ? 0 : have;
@@ -39,19 +39,14 @@ __device__ __forceinline__ int page_ok(const PagedRows& r, int page) {
     return -1;
 }
 
-// Row of the cache (in units of [K | V] rows) that holds packed row `tok` of kv head `head`, -1: none.
-__device__ __forceinline__ int64_t cache_row(const PagedRows& r, int tok, int head) {
-    int lo = 0, hi = r.B;            // the first sequence that ends behind tok
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (r.cu[mid + 1] <= tok) lo = mid + 1;
-        else hi = mid;
-    }
-    if (lo >= r.B || r.cu[lo] > tok) return -1;
-    const int pos = cached(r, lo) - min(r.cu[lo + 1], r.T) + tok;
-    if (pos < 0) return -1;
-    const int page = page_ok(r, r.table[(int64_t)lo * r.P + (pos >> r.shift)]);
-    return page < 0 ? -1 : ((((int64_t)page * r.Hkv + head) << r.shift) | (pos & ((1 << r.shift) - 1)));
+// e4m3 pairs -> bf16 pairs times a power of two
+__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float s) {
+    u32x4 w;
+    w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));
+    w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true));
+    w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false));
+    w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
+    return w;
 }
 
 // bits of the largest magnitude over the D / 8 lanes that share a row (non-negative numbers order as their bits do)
@@ -71,62 +66,130 @@ struct CopyArgs {
     uint16_t *ko, *vo;                           // read: out, contiguous
     char* pool;
     uint8_t* scale;
+    int per_block;                               // tokens a workgroup copies
 };
 
-// One lane carries 8 elements (16 bytes of bf16); a row is D / 8 neighbouring lanes, K and V of a (token, head) neighbouring rows.
-// Bound by memory: 4 D bytes in and 4 D (e4m3: 2 D + 2) out per token and kv head.
+constexpr int COPY_TOKENS = 32;                  // at most
+constexpr int COPY_SEQS = 255;                   // requests whose lengths a workgroup keeps in LDS
+constexpr uint32_t NO_ROW = 0xffffffffu;
+
+// Rows in (READ false) and out.  A workgroup takes `per_block` tokens, finds their places once, one thread a token, and then
+// streams all their heads, 16 bytes of bf16 a lane and COPY_UNROLL of them in flight: a row is D / 8 neighbouring lanes, K and V
+// of a (token, head) neighbouring rows.  Bound by memory: 4 D bytes in and 4 D (e4m3: 2 D + 2) out per token and kv
+// head.
+constexpr int COPY_UNROLL = 4;
 template <int D, bool E4M3, bool READ>
 __global__ __launch_bounds__(256) void paged_copy_kernel(const CopyArgs a) {
     constexpr int LANES = D / 8;
-    const int64_t idx = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    const int c = threadIdx.x % LANES, which = (int)(idx & 1);
-    const int64_t th = idx >> 1;
-    if (th >= (int64_t)a.r.T * a.r.Hkv) return;
-    const int tok = (int)(th / a.r.Hkv), head = (int)(th % a.r.Hkv);
-    const int64_t row = cache_row(a.r, tok, head);
-    if (row < 0) return;
-    if (READ) {
-        uint16_t* out = (which ? a.vo : a.ko) + th * D + 8 * c;
-        if (!E4M3) {
-            *reinterpret_cast<u32x4*>(out) = *reinterpret_cast<const u32x4*>(a.pool + ((row * 2 + which) * LANES + c) * 16);
-        } else {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(a.pool + ((row * 2 + which) * LANES + c) * 8);
-            const float s = __uint_as_float((uint32_t)a.scale[row * 2 + which] << 23);
-            u32x4 o;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], s, false));
-                o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], s, true));
-            }
-            *reinterpret_cast<u32x4*>(out) = o;
+    __shared__ uint32_t place[COPY_TOKENS];
+    __shared__ int s_cu[COPY_SEQS + 1], s_kv[COPY_SEQS];
+    const PagedRows& r = a.r;
+    const int t0 = blockIdx.x * a.per_block, tokens = min(a.per_block, r.T - t0);
+    const bool small = r.B <= COPY_SEQS;
+    if (small) {
+        if ((int)threadIdx.x <= r.B) s_cu[threadIdx.x] = r.cu[threadIdx.x];
+        if ((int)threadIdx.x < r.B) s_kv[threadIdx.x] = r.kv_len[threadIdx.x];
+        __syncthreads();
+    }
+    if ((int)threadIdx.x < tokens) {
+        const int tok = t0 + threadIdx.x;
+        auto cu = [&](int i) { return small ? s_cu[i] : r.cu[i]; };
+        int lo = 0, hi = r.B;                    // the first request that ends behind tok
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (cu(mid + 1) <= tok) lo = mid + 1;
+            else hi = mid;
         }
-        return;
+        uint32_t at = NO_ROW;
+        if (lo < r.B && cu(lo) <= tok) {
+            const int pos = cached(r, small ? s_kv[lo] : r.kv_len[lo]) - min(cu(lo + 1), r.T) + tok;
+            if (pos >= 0) {
+                const int page = page_ok(r, r.table[(int64_t)lo * r.P + (pos >> r.shift)]);
+                if (page >= 0) at = (((uint32_t)page * (uint32_t)r.Hkv) << r.shift) | (uint32_t)(pos & ((1 << r.shift) - 1));
+            }
+        }
+        place[threadIdx.x] = at;
     }
-    const uint16_t* in = which ? a.v + tok * a.v_st + head * a.v_sh : a.k + tok * a.k_st + head * a.k_sh;
-    const u32x4 x = *reinterpret_cast<const u32x4*>(in + 8 * c);
-    if (!E4M3) {
-        *reinterpret_cast<u32x4*>(a.pool + ((row * 2 + which) * LANES + c) * 16) = x;
-        return;
-    }
-    uint32_t top = 0;
+    __syncthreads();
+    const int per_token = 2 * r.Hkv * LANES;     // 16-byte pieces
+    const int step_t = 256 / per_token, step_c = 256 % per_token;
+    int tl = (int)threadIdx.x / per_token, c = (int)threadIdx.x % per_token;
+    while (__any(tl < tokens)) {
+        const uint16_t* in[COPY_UNROLL];
+        uint32_t row[COPY_UNROLL];
+        int tc[COPY_UNROLL], cc[COPY_UNROLL];
+        u32x4 x[COPY_UNROLL];
+        uint32_t e[COPY_UNROLL];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = x[i] & 0x7fffu, hi = (x[i] >> 16) & 0x7fffu;
-        top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-    }
-    top = row_lanes_max<D>(top);
-    // exponent - 127 - 8, one more where the mantissa is above 1.75 = 448 / 2^8; as a biased exponent, at least 1
-    const int e = max((int)(top >> 7) - 8 + ((top & 127u) > 96u ? 1 : 0), 1);
-    const float up = __uint_as_float((uint32_t)(254 - e) << 23);
-    u32x2 w;
+        for (int u = 0; u < COPY_UNROLL; ++u) {
+            tc[u] = tl;
+            cc[u] = c;
+            row[u] = NO_ROW;
+            if (tl < tokens) {
+                const uint32_t at = place[tl];
+                if (at != NO_ROW) row[u] = at + ((uint32_t)(c / (2 * LANES)) << r.shift);
+            }
+            tl += step_t;
+            c += step_c;
+            if (c >= per_token) {
+                c -= per_token;
+                ++tl;
+            }
+        }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        int word = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(x[2 * i]) * up, bf16_hi(x[2 * i]) * up, 0, false);
-        word = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(x[2 * i + 1]) * up, bf16_hi(x[2 * i + 1]) * up, word, true);
-        w[i] = (uint32_t)word;
+        for (int u = 0; u < COPY_UNROLL; ++u) {
+            const int head = cc[u] / (2 * LANES), which = (cc[u] / LANES) & 1, p = cc[u] % LANES;
+            if (row[u] == NO_ROW) continue;
+            const uint64_t w = (uint64_t)row[u] * 2 + which;
+            if (READ) {
+                if (E4M3) {
+                    const u32x2 y = *reinterpret_cast<const u32x2*>(a.pool + (w * LANES + p) * 8);
+                    x[u][0] = y[0];
+                    x[u][1] = y[1];
+                    e[u] = a.scale[w];
+                } else {
+                    x[u] = *reinterpret_cast<const u32x4*>(a.pool + (w * LANES + p) * 16);
+                }
+            } else {
+                const int64_t tok = t0 + tc[u];
+                in[u] = which ? a.v + tok * a.v_st + head * a.v_sh : a.k + tok * a.k_st + head * a.k_sh;
+                x[u] = *reinterpret_cast<const u32x4*>(in[u] + 8 * p);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < COPY_UNROLL; ++u) {
+            const int head = cc[u] / (2 * LANES), which = (cc[u] / LANES) & 1, p = cc[u] % LANES;
+            if (row[u] == NO_ROW) continue;
+            const uint64_t w = (uint64_t)row[u] * 2 + which;
+            if (READ) {
+                uint16_t* out = (which ? a.vo : a.ko) + ((int64_t)(t0 + tc[u]) * r.Hkv + head) * D + 8 * p;
+                if (E4M3) x[u] = widen8(x[u][0], x[u][1], __uint_as_float(e[u] << 23));
+                *reinterpret_cast<u32x4*>(out) = x[u];
+            } else if (!E4M3) {
+                *reinterpret_cast<u32x4*>(a.pool + (w * LANES + p) * 16) = x[u];
+            } else {
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t l = x[u][i] & 0x7fffu, h = (x[u][i] >> 16) & 0x7fffu;
+                    top = max(top, max(l < 0x7f80u ? l : 0u, h < 0x7f80u ? h : 0u));
+                }
+                top = row_lanes_max<D>(top);
+                // exponent - 127 - 8, one more where the mantissa is above 1.75 = 448 / 2^8; as a biased exponent, at least 1
+                const int ex = max((int)(top >> 7) - 8 + ((top & 127u) > 96u ? 1 : 0), 1);
+                const float up = __uint_as_float((uint32_t)(254 - ex) << 23);
+                u32x2 y;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    int word = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(x[u][2 * i]) * up, bf16_hi(x[u][2 * i]) * up, 0, false);
+                    word = __builtin_amdgcn_cvt_pk_fp8_f32(bf16_lo(x[u][2 * i + 1]) * up, bf16_hi(x[u][2 * i + 1]) * up, word, true);
+                    y[i] = (uint32_t)word;
+                }
+                *reinterpret_cast<u32x2*>(a.pool + (w * LANES + p) * 8) = y;
+                if (p == 0) a.scale[w] = (uint8_t)ex;
+            }
+        }
     }
-    *reinterpret_cast<u32x2*>(a.pool + ((row * 2 + which) * LANES + c) * 8) = w;
-    if (c == 0) a.scale[row * 2 + which] = (uint8_t)e;
 }
 
 // ---------------------------------------------------------------- attention over the pages
@@ -165,7 +228,7 @@ __device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units
     p.start = p.n = p.row0 = p.kv = p.part = 0;
     auto first = [&](int i) { return min(max(r.cu[i], 0), r.T); };
     auto row_tiles = [&](int i) { return (max(first(i + 1) - first(i), 0) * G + BM - 1) / BM; };
-    auto key_tiles = [&](int i) { return (int)(((int64_t)cached(r, i) + TOK - 1) / TOK); };
+    auto key_tiles = [&](int i) { return (int)(((int64_t)cached(r, r.kv_len[i]) + TOK - 1) / TOK); };
     p.per = 0x7fffffff;
     if (units > 0) {
         float work = 0.f;            // (products of large counts; the quotient need not be exact)
@@ -189,7 +252,7 @@ __device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units
             p.seq = base + k;
             p.start = first(p.seq);
             p.n = first(p.seq + 1) - p.start;
-            p.kv = cached(r, p.seq);
+            p.kv = cached(r, r.kv_len[p.seq]);
             p.row0 = at / np * BM;
             p.part = at % np;
             return p;
@@ -197,16 +260,6 @@ __device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units
         before = __builtin_amdgcn_readlane(sum, WAVE - 1);
     }
     return p;
-}
-
-// e4m3 pairs -> bf16 pairs times a power of two
-__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float s) {
-    u32x4 w;
-    w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));
-    w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true));
-    w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false));
-    w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
-    return w;
 }
 
 // Many rows: 128 of one (request, kv head) a workgroup, everything else as in prompt.hip.  An e4m3 tile passes through
@@ -516,9 +569,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 }
 
 // ---------------------------------------------------------------- host
-int64_t paged_copy_grid(int64_t T, int Hkv, int D) {
-    const int rows = 256 / (D / 8);
-    return (T * Hkv * 2 + rows - 1) / rows;
+// Tokens a workgroup copies: one pass of its threads, and from 2048 tokens on as many as leave a CU eight workgroups (fewer
+// lookups).
+static int copy_tokens(int64_t T, int Hkv, int D) {
+    const int64_t pass = 256 / (Hkv * D / 4), n = T / 2048 > pass ? T / 2048 : pass;
+    return n < 1 ? 1 : n > COPY_TOKENS ? COPY_TOKENS : (int)n;
 }
 
 static PagedRows paged_rows(const int32_t* cu, int B, int T, const int32_t* table, int P, const int32_t* kv_len, int shift,
@@ -528,7 +583,7 @@ static PagedRows paged_rows(const int32_t* cu, int B, int T, const int32_t* tabl
 
 template <int D>
 static void paged_copy(const CopyArgs& a, bool e4m3, bool read, hipStream_t st) {
-    const dim3 grid((unsigned)paged_copy_grid(a.r.T, a.r.Hkv, D));
+    const dim3 grid((unsigned)((a.r.T + a.per_block - 1) / a.per_block));
     if (e4m3) {
         if (read) paged_copy_kernel<D, true, true><<<grid, 256, 0, st>>>(a);
         else paged_copy_kernel<D, true, false><<<grid, 256, 0, st>>>(a);
@@ -542,7 +597,7 @@ hipError_t launch_paged_append(const uint16_t* k, int64_t k_st, int64_t k_sh, co
                                const int32_t* cu, int B, int T, const int32_t* table, int P, const int32_t* kv_len, int shift,
                                int num_pages, int Hkv, int D, bool e4m3, char* pool, uint8_t* scale, int* err, hipStream_t st) {
     const CopyArgs a{paged_rows(cu, B, T, table, P, kv_len, shift, num_pages, Hkv, err), k, v, k_st, k_sh, v_st, v_sh,
-                     nullptr, nullptr, pool, scale};
+                     nullptr, nullptr, pool, scale, copy_tokens(T, Hkv, D)};
     if (D == 128) paged_copy<128>(a, e4m3, false, st);
     else paged_copy<64>(a, e4m3, false, st);
     return hipGetLastError();
@@ -552,7 +607,7 @@ hipError_t launch_paged_read(uint16_t* k, uint16_t* v, const int32_t* cu, int B,
                              const int32_t* kv_len, int shift, int num_pages, int Hkv, int D, bool e4m3, char* pool,
                              uint8_t* scale, int* err, hipStream_t st) {
     const CopyArgs a{paged_rows(cu, B, T, table, P, kv_len, shift, num_pages, Hkv, err), nullptr, nullptr, 0, 0, 0, 0,
-                     k, v, pool, scale};
+                     k, v, pool, scale, copy_tokens(T, Hkv, D)};
     if (D == 128) paged_copy<128>(a, e4m3, true, st);
     else paged_copy<64>(a, e4m3, true, st);
     return hipGetLastError();

@@ -22,6 +22,7 @@ from .prompt_attention import rows_strides, same_device
 class PagedKVCache:
     def __init__(self):
         self._h = C.c_void_p()
+        self._sizes = {}                       # workspace bytes by the sizes of a call
         L.check(L.lib().mp_paged_create(C.byref(self._h)))
 
     def __del__(self):
@@ -53,30 +54,34 @@ class PagedKVCache:
         L.expect(page_table, torch.int32, (B, P), "page_table")
         L.expect(cu_seqlens, torch.int32, (B + 1,), "cu_seqlens")
         L.expect(kv_len, torch.int32, (B,), "kv_len")
-        same_device(torch.device("cuda", self._device), cu_seqlens=cu_seqlens, page_table=page_table, kv_len=kv_len, **tensors)
-        return (L.ptr(cu_seqlens), B, num_tokens, L.ptr(page_table), P, L.ptr(kv_len))
+        same_device(self._device, cu_seqlens=cu_seqlens, page_table=page_table, kv_len=kv_len, **tensors)
+        return cu_seqlens.data_ptr(), B, num_tokens, page_table.data_ptr(), P, kv_len.data_ptr()
 
     def append(self, layer_id: int, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor,
                kv_len: torch.Tensor) -> None:
         """k, v bf16 [T, Hkv, D] (any token / head strides that are multiples of 8 elements) into the pages: row
         cu_seqlens[b] + i becomes position kv_len[b] - n_b + i of request b, n_b its number of new rows."""
-        ks, vs = rows_strides(k, self.Hkv, self.D, "k"), rows_strides(v, self.Hkv, self.D, "v")
-        if k.shape[0] != v.shape[0]:
-            raise ValueError(f"k, v: {k.shape[0]} and {v.shape[0]} tokens")
-        rows = self._rows(k.shape[0], cu_seqlens, page_table, kv_len, k=k, v=v)
-        L.check(L.lib().mp_paged_append(self._h, layer_id, L.ptr(k), *ks, L.ptr(v), *vs, *rows,
-                                        L.current_stream(device=self._device)))
+        (T, kt, kh), (Tv, vt, vh) = rows_strides(k, self.Hkv, self.D, "k"), rows_strides(v, self.Hkv, self.D, "v")
+        if T != Tv:
+            raise ValueError(f"k, v: {T} and {Tv} tokens")
+        rows = self._rows(T, cu_seqlens, page_table, kv_len, k=k, v=v)
+        L.check(L.lib().mp_paged_append(self._h, layer_id, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, *rows,
+                                        L.stream_on(self._device)))
 
     def read(self, layer_id: int, num_tokens: int, cu_seqlens: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor,
              k: torch.Tensor | None = None, v: torch.Tensor | None = None):
         """The rows append would write for this description, out of the pages: (k, v) bf16 [num_tokens, Hkv, D]."""
         shape = (num_tokens, self.Hkv, self.D)
-        k = torch.empty(shape, dtype=torch.bfloat16, device=kv_len.device) if k is None else k
-        v = torch.empty(shape, dtype=torch.bfloat16, device=kv_len.device) if v is None else v
+        rows = self._rows(num_tokens, cu_seqlens, page_table, kv_len)
+        if k is None:
+            k = page_table.new_empty(shape, dtype=torch.bfloat16)
+        if v is None:
+            v = page_table.new_empty(shape, dtype=torch.bfloat16)
         L.expect(k, torch.bfloat16, shape, "k")
         L.expect(v, torch.bfloat16, shape, "v")
-        rows = self._rows(num_tokens, cu_seqlens, page_table, kv_len, k=k, v=v)
-        L.check(L.lib().mp_paged_read(self._h, layer_id, L.ptr(k), L.ptr(v), *rows, L.current_stream(device=self._device)))
+        same_device(self._device, k=k, v=v)
+        L.check(L.lib().mp_paged_read(self._h, layer_id, k.data_ptr(), v.data_ptr(), *rows,
+                                      L.stream_on(self._device)))
         return k, v
 
     def attention(self, layer_id: int, q: torch.Tensor, cu_seqlens: torch.Tensor, page_table: torch.Tensor,
@@ -85,27 +90,40 @@ class PagedKVCache:
         """q bf16 [T, H, D]: row cu_seqlens[b] + i attends to positions 0 .. kv_len[b] - n_b + i of request b, as the pages hold
         them (append the rows' own keys first); query head h to kv head h // (H // Hkv).  Returns (out bf16 [T, H, D],
         lse f32 [T, H], base 2); a row that sees nothing gives 0 and -inf.  scale: default head_dim ** -0.5."""
-        qs = rows_strides(q, self.H, self.D, "q")
-        T = q.shape[0]
+        H, D = self.H, self.D
+        T, qt, qh = rows_strides(q, H, D, "q")
         if out is None:
-            out = torch.empty((T, self.H, self.D), dtype=torch.bfloat16, device=q.device)
+            out = q.new_empty((T, H, D))
+        else:
+            L.expect(out, torch.bfloat16, (T, H, D), "out")
         if lse is None:
-            lse = torch.empty((T, self.H), dtype=torch.float32, device=q.device)
-        L.expect(out, torch.bfloat16, (T, self.H, self.D), "out")
-        L.expect(lse, torch.float32, (T, self.H), "lse")
+            lse = q.new_empty((T, H), dtype=torch.float32)
+        else:
+            L.expect(lse, torch.float32, (T, H), "lse")
         rows = self._rows(T, cu_seqlens, page_table, kv_len, q=q, out=out, lse=lse)
-        need = C.c_int64()
-        L.check(L.lib().mp_paged_workspace(self._h, rows[1], T, rows[4], C.byref(need)))
+        size = self._workspace(rows[1], T, rows[4])
         # from torch's allocator: safe to reuse in stream order, and a captured graph's own
-        work = torch.empty((need.value,), dtype=torch.uint8, device=q.device) if need.value else None
-        L.check(L.lib().mp_paged_attention(self._h, layer_id, L.ptr(q), *qs, *rows, self.D ** -0.5 if scale is None else float(scale),
-                                           L.ptr(out), L.ptr(lse), L.ptr(work), need.value,
-                                           L.current_stream(device=self._device)))
+        work = q.new_empty((size,), dtype=torch.uint8) if size else None
+        L.check(L.lib().mp_paged_attention(self._h, layer_id, q.data_ptr(), qt, qh, *rows, D ** -0.5 if scale is None else float(scale),
+                                           out.data_ptr(), lse.data_ptr(), L.ptr(work), size,
+                                           L.stream_on(self._device)))
         return out, lse
+
+    def _workspace(self, requests: int, tokens: int, pages: int) -> int:
+        """mp_paged_workspace: bytes, by the sizes alone."""
+        key = (requests, tokens, pages)
+        size = self._sizes.get(key)
+        if size is None:
+            need = C.c_int64()
+            L.check(L.lib().mp_paged_workspace(self._h, requests, tokens, pages, C.byref(need)))
+            if len(self._sizes) >= 4096:
+                self._sizes.clear()
+            size = self._sizes[key] = need.value
+        return size
 
     def check(self) -> None:
         """Raise if a call since the last check met a page id or length outside the cache (waits for the current stream)."""
-        L.check(L.lib().mp_paged_check(self._h, L.current_stream(device=self._device)))
+        L.check(L.lib().mp_paged_check(self._h, L.stream_on(self._device)))
 
     def get_pages(self, layer_id: int):
         """Views of the handle's memory: pages [num_pages, Hkv, page_size, 2 (K, V), D] in bf16 or float8_e4m3fn, and the rows'

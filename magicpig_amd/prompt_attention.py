@@ -9,8 +9,16 @@ from . import _lib as L
 
 
 def rows_strides(t: torch.Tensor, heads: int, head_dim: int, name: str):
-    """Checks a bf16 CUDA tensor [tokens, heads, head_dim] whose dims are contiguous; returns its token and head stride
-    (those of an axis of length 1, which torch leaves arbitrary, as if it were contiguous)."""
+    """Checks a bf16 CUDA tensor [tokens, heads, head_dim] whose dims are contiguous; returns its tokens, token and head
+    stride (the strides of an axis of length 1, which torch leaves arbitrary, as if it were contiguous)."""
+    try:      # the common case first (the host's share of a small call is larger than the kernel's)
+        n, h, d = t.shape
+        if t.dtype is torch.bfloat16 and h == heads and d == head_dim and t.is_cuda:
+            st, sh, sd = t.stride()
+            if sd == 1:
+                return n, st if n > 1 else heads * head_dim, sh if heads > 1 else head_dim
+    except (AttributeError, ValueError):
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype is not torch.bfloat16:
@@ -19,16 +27,13 @@ def rows_strides(t: torch.Tensor, heads: int, head_dim: int, name: str):
         raise ValueError(f"{name}: expected shape (tokens, {heads}, {head_dim}), got {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor")
-    if t.stride(2) != 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
-    head = t.stride(1) if heads > 1 else head_dim
-    return (t.stride(0) if t.shape[0] > 1 else heads * head_dim), head
+    raise ValueError(f"{name}: the last dimension must be contiguous")
 
 
-def same_device(device: torch.device, **tensors) -> None:
+def same_device(index: int, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name}: on {t.device}, expected {device}")
+        if t.get_device() != index:
+            raise ValueError(f"{name}: on {t.device}, expected cuda:{index}")
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, scale: float | None = None,
@@ -40,26 +45,32 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     `lse` where their contents matter.  head_dim 64 or 128.  Runs on torch's current stream of q's device."""
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise ValueError("q: expected a tensor [tokens, heads, head_dim]")
-    T, H, D = q.shape
     if not isinstance(k, torch.Tensor) or k.dim() != 3:
         raise ValueError("k: expected a tensor [tokens, heads, head_dim]")
+    _, H, D = q.shape
     Hkv = k.shape[1]
-    qs = rows_strides(q, H, D, "q")
-    ks, vs = rows_strides(k, Hkv, D, "k"), rows_strides(v, Hkv, D, "v")
-    if k.shape[0] != T or v.shape[0] != T:
-        raise ValueError(f"k, v: expected {T} tokens, got {k.shape[0]} and {v.shape[0]}")
+    T, qt, qh = rows_strides(q, H, D, "q")
+    (Tk, kt, kh), (Tv, vt, vh) = rows_strides(k, Hkv, D, "k"), rows_strides(v, Hkv, D, "v")
+    if Tk != T or Tv != T:
+        raise ValueError(f"k, v: expected {T} tokens, got {Tk} and {Tv}")
     if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
         raise ValueError("cu_seqlens: expected a tensor [sequences + 1]")
     L.expect(cu_seqlens, torch.int32, cu_seqlens.shape, "cu_seqlens")
     if out is None:
-        out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((T, H, D))
+    else:
+        L.expect(out, torch.bfloat16, (T, H, D), "out")
     if lse is None:
-        lse = torch.empty((T, H), dtype=torch.float32, device=q.device)
-    L.expect(out, torch.bfloat16, (T, H, D), "out")
-    L.expect(lse, torch.float32, (T, H), "lse")
-    same_device(q.device, k=k, v=v, cu_seqlens=cu_seqlens, out=out, lse=lse)
-    with torch.cuda.device(q.device):                    # no handle: launch where the data is
-        L.check(L.lib().mp_prompt_attention(
-            L.ptr(q), *qs, L.ptr(k), *ks, L.ptr(v), *vs, L.ptr(cu_seqlens), cu_seqlens.shape[0] - 1, T, H, Hkv, D,
-            D ** -0.5 if scale is None else float(scale), L.ptr(out), L.ptr(lse), L.current_stream(q)))
+        lse = q.new_empty((T, H), dtype=torch.float32)
+    else:
+        L.expect(lse, torch.float32, (T, H), "lse")
+    device = q.get_device()
+    same_device(device, k=k, v=v, cu_seqlens=cu_seqlens, out=out, lse=lse)
+    args = (q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, T,
+            H, Hkv, D, D ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr(), L.stream_on(device))
+    if device == torch.cuda.current_device():
+        L.check(L.lib().mp_prompt_attention(*args))
+    else:
+        with torch.cuda.device(device):                  # no handle: launch where the data is
+            L.check(L.lib().mp_prompt_attention(*args))
     return out, lse
