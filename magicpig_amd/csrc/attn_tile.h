@@ -7,10 +7,12 @@
 // Mathematics.  For a row with visible keys 0 .. lim the kernels fold the tokens in once, tile by tile:
 //     s_j = q . k_j (f32 accumulation of exact bf16 products),  x_j = c s_j,  c = scale log2(e)
 //     m' = max(m, max_j x_j),  l' = 2^(m - m') l + sum_j 2^(x_j - m'),  o' = 2^(m - m') o + sum_j 2^(x_j - m') v_j
-// and end with o / l and the base-2 log-sum-exp m + log2 l.  m only moves when a tile's maximum lies more than
-// 8 above it (2^8 times larger weights change neither f32 sums nor the relative precision of a bf16 weight), so
-// most tiles rescale nothing.  m, l, o are f32; the weights 2^(x - m) are rounded to bf16 once, for the second
-// matrix product (relative error 2^-9 each, the rounding the output gets anyway); l sums them unrounded.
+// and end with o / l and the base-2 log-sum-exp m + log2 l.  m need not be the maximum, only near or above it: the weights
+// are made with the m there is, and only where a lane's share of a tile's weights sums to more than 1024 (or the row has seen
+// nothing yet) is the maximum looked for, m moved, o and l scaled and the weights made again.  Larger weights change neither f32
+// sums nor the relative precision of a bf16 weight, and most tiles cost no maximum and no scaling (3 % at 32 768 tokens).
+// m, l, o are f32; the weights 2^(x - m) are rounded to bf16 once, for the second matrix product (relative error 2^-8 each at
+// most, as the output's own rounding); l sums them unrounded.
 //
 // Lanes.  Both products are v_mfma_f32_32x32x16_bf16.  The first computes S^T = K Q^T: lane l holds column
 // (row of q) l % 32 and, of 32 tokens, the 16 with (t >> 2) & 1 == l / 32.  So a row's maximum and sum are sums over a
@@ -36,7 +38,7 @@ typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 constexpr int TILE_TOKENS = 64;         // tokens staged at a time
 constexpr float NEG_INF = -__builtin_inff();
-constexpr float LAZY_MAX = 8.f;         // see above: how far a maximum may lie above m before m follows
+constexpr float LAZY_SUM = 1024.f;       // see above
 
 template <int D>
 __device__ __forceinline__ int key_swizzle(int row) { return D == 128 ? (row & 15) : ((row >> 1) & 7); }
@@ -166,12 +168,11 @@ __device__ __forceinline__ void add_nonfinite(f32x16 (&o)[D / 32], const char* v
     }
 }
 
-// Fold SUB * 32 tokens (K rows at kt, V rows at vt in LDS) into the wave's rows.  MASK: only tokens <= lim (relative to the
-// tile, per lane) are visible to the lane's row.
-template <int D, int SUB, bool MASK>
-__device__ __forceinline__ void fold_tile(RowState<D>& st, const char* kt, const char* vt, float c, int lim) {
+// The steps of folding SUB * 32 tokens (K rows at kt, V rows at vt in LDS) into the wave's rows.
+// s = K Q^T
+template <int D, int SUB>
+__device__ __forceinline__ void tile_scores(f32x16 (&s)[SUB], const RowState<D>& st, const char* kt) {
     const int l = lane_id(), h = l >> 5, row = l & 31;
-    f32x16 s[SUB];
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -183,31 +184,38 @@ __device__ __forceinline__ void fold_tile(RowState<D>& st, const char* kt, const
             const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kt + (32 * u + row) * (2 * D) + (((2 * k + h) ^ key_swizzle<D>(row)) << 4));
             s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, st.q[k], s[u], 0, 0, 0);
         }
-    if (MASK) {
+}
+// only tokens <= lim (relative to the tile, per lane) are visible to the lane's row
+template <int SUB>
+__device__ __forceinline__ void mask_scores(f32x16 (&s)[SUB], int lim) {
+    const int h = lane_id() >> 5;
 #pragma unroll
-        for (int u = 0; u < SUB; ++u)
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (32 * u + 8 * (r >> 2) + 4 * h + (r & 3) > lim) s[u][r] = NEG_INF;
-    }
+        for (int r = 0; r < 16; ++r)
+            if (32 * u + 8 * (r >> 2) + 4 * h + (r & 3) > lim) s[u][r] = NEG_INF;
+}
+// m follows these scores
+template <int D, int SUB>
+__device__ __forceinline__ void move_maximum(RowState<D>& st, const f32x16 (&s)[SUB], float c) {
     float top = s[0][0];
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-    top = halves_max(top) * c;
-    if (__ballot(top > st.m + LAZY_MAX)) {               // (-inf + 8 = -inf: a row's first visible tile always enters)
-        const float m = fmaxf(st.m, top);
-        const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
-        st.m = m;
-        st.l *= f;
+    const float m = fmaxf(st.m, halves_max(top) * c);
+    const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f(st.m - m);
+    st.m = m;
+    st.l *= f;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
+    for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) st.o[i][r] *= f;
-    }
+        for (int r = 0; r < 16; ++r) st.o[i][r] *= f;
+}
+// p = 2^(c s - m); returns their sum
+template <int D, int SUB>
+__device__ __forceinline__ float tile_weights(const RowState<D>& st, const f32x16 (&s)[SUB], float c, bf16x8 (&p)[2 * SUB]) {
     const float off = st.m == NEG_INF ? 0.f : st.m;      // nothing seen yet: every weight below is 2^-inf = 0
-    bf16x8 p[2 * SUB];
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
@@ -217,7 +225,20 @@ __device__ __forceinline__ void fold_tile(RowState<D>& st, const char* kt, const
             sum += w;
             p[2 * u + (r >> 3)][r & 7] = (__bf16)w;
         }
+    return sum;
+}
+// ... taken over, or made again from a maximum that follows
+template <int D, int SUB>
+__device__ __forceinline__ void settle_weights(RowState<D>& st, const f32x16 (&s)[SUB], float c, bf16x8 (&p)[2 * SUB], float sum) {
+    if (__ballot(sum > LAZY_SUM || st.m == NEG_INF)) {
+        move_maximum<D, SUB>(st, s, c);
+        sum = tile_weights<D, SUB>(st, s, c, p);
+    }
     st.l += sum;
+}
+// o += V^T p
+template <int D, int SUB, bool MASK>
+__device__ __forceinline__ void add_values(RowState<D>& st, const bf16x8 (&p)[2 * SUB], const char* vt, int lim) {
     const bool odd = MASK && tile_has_nonfinite<D, SUB>(vt);
 #pragma unroll
     for (int t = 0; t < 2 * SUB; ++t) {
@@ -230,6 +251,16 @@ __device__ __forceinline__ void fold_tile(RowState<D>& st, const char* kt, const
         }
     }
     if (MASK && odd) add_nonfinite<D, SUB>(st.o, vt, lim);
+}
+template <int D, int SUB, bool MASK>
+__device__ __forceinline__ void fold_tile(RowState<D>& st, const char* kt, const char* vt, float c, int lim) {
+    f32x16 s[SUB];
+    bf16x8 p[2 * SUB];
+    tile_scores<D, SUB>(s, st, kt);
+    if (MASK) mask_scores<SUB>(s, lim);
+    const float sum = tile_weights<D, SUB>(st, s, c, p);
+    settle_weights<D, SUB>(st, s, c, p, sum);
+    add_values<D, SUB, MASK>(st, p, vt, lim);
 }
 
 // Which sequence and which of its tiles a slot is.  Sequence b of rows cu[b] G .. cu[b + 1] G owns the slots from

@@ -1,8 +1,8 @@
 // prompt.hip -- causal attention over whole prompts packed one behind the other, query heads in groups.
 //
-// A workgroup owns 128 rows (see attn_tile.h: a row is one query head of one token, the G heads of a kv head
+// A workgroup owns 128 or 256 rows (see attn_tile.h: a row is one query head of one token, the G heads of a kv head
 // side by side) of one (sequence, kv head) and walks the sequence's keys in tiles of 64 tokens, two buffers in LDS:
-// while tile j is folded in, the DMA engine fetches tile j + 1.  Its four waves hold 32 rows each.
+// while tile j is folded in, the DMA engine fetches tile j + 1.  Its waves hold 32 rows each.
 #include "attn_tile.h"
 
 namespace mp {
@@ -17,9 +17,16 @@ struct PromptArgs {
     float* lse;
 };
 
-template <int D>
-__global__ __launch_bounds__(256, 2) void prompt_attention_kernel(const PromptArgs a) {
-    constexpr int BM = 128, CPR = D / 8, PASSES = TILE_TOKENS * CPR / 256, KB = TILE_TOKENS * 2 * D;
+// Rows of a workgroup at head_dim 128.  256 rows read every key tile from L2 half as often: 16 384 tokens of 8 heads over one
+// kv head 511 us against 551, 32 768 tokens of 32 heads over 8 7.88 ms against 8.01.  They need 2^17 rows to give every CU two
+// workgroups (8192 tokens of 8 heads: 205 us against 178), and long sequences, whose last workgroup is not a large part of the
+// whole (8 sequences of 1000, 32 heads: 101 us against 97).  At head_dim 64 three workgroups of 128 rows fit a CU and one
+// of 256 (8100 tokens, 32 heads: 182 us against 167).
+constexpr int64_t WIDE_ROWS = 1 << 17, WIDE_TOKENS = 2048;
+
+template <int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const PromptArgs a) {
+    constexpr int THREADS = 64 * WAVES, BM = 32 * WAVES, CPR = D / 8, PASSES = TILE_TOKENS * CPR / THREADS, KB = TILE_TOKENS * 2 * D;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][KB];      // [buffer][K, V]
     // heads fastest: with 8 kv heads the workgroups of one head meet in one XCD's L2; longest rows of a sequence first
     const int head = blockIdx.x % a.Hkv;
@@ -47,10 +54,10 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(const PromptAr
         const int last = t.n - 1 - tile * TILE_TOKENS;                  // behind the end: the last token again, masked
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            const int idx = i * 256 + (int)threadIdx.x, r = idx / CPR, p = idx % CPR;
+            const int idx = i * THREADS + (int)threadIdx.x, r = idx / CPR, p = idx % CPR;
             const uint32_t s = (uint32_t)min(r, last);
-            dma16(kt + (s * kst + ((p ^ key_swizzle<D>(r)) << 4)), lds[tile & 1][0] + (i * 256 + w * 64) * 16);
-            dma16(vt + (s * vst + ((p ^ value_swizzle<D>(r)) << 4)), lds[tile & 1][1] + (i * 256 + w * 64) * 16);
+            dma16(kt + (s * kst + ((p ^ key_swizzle<D>(r)) << 4)), lds[tile & 1][0] + (i * THREADS + w * 64) * 16);
+            dma16(vt + (s * vst + ((p ^ value_swizzle<D>(r)) << 4)), lds[tile & 1][1] + (i * THREADS + w * 64) * 16);
         }
     };
     stage(0);
@@ -72,14 +79,19 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_kernel(const PromptAr
 
 int64_t prompt_grid(int64_t T, int B, int G, int Hkv) { return (T * G / 128 + B) * Hkv; }
 
+template <int D, int WAVES>
+static void prompt_attention(PromptArgs a, hipStream_t st) {
+    a.slots = (int)((int64_t)a.T * a.G / (32 * WAVES) + a.B);
+    prompt_attention_kernel<D, WAVES><<<dim3((unsigned)(a.slots * a.Hkv)), 64 * WAVES, 0, st>>>(a);
+}
+
 hipError_t launch_prompt_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, const uint16_t* k, int64_t k_st,
                                    int64_t k_sh, const uint16_t* v, int64_t v_st, int64_t v_sh, const int32_t* cu, int B,
                                    int T, int H, int Hkv, int D, float c, uint16_t* out, float* lse, hipStream_t st) {
-    const int G = H / Hkv;
-    const PromptArgs a{q, k, v, q_st, q_sh, k_st, k_sh, v_st, v_sh, cu, B, T, H, Hkv, G, (int)((int64_t)T * G / 128 + B), c, out, lse};
-    const dim3 grid((unsigned)prompt_grid(T, B, G, Hkv));
-    if (D == 128) prompt_attention_kernel<128><<<grid, 256, 0, st>>>(a);
-    else prompt_attention_kernel<64><<<grid, 256, 0, st>>>(a);
+    const PromptArgs a{q, k, v, q_st, q_sh, k_st, k_sh, v_st, v_sh, cu, B, T, H, Hkv, H / Hkv, 0, c, out, lse};
+    if (D == 64) prompt_attention<64, 4>(a, st);
+    else if ((int64_t)T * H >= WIDE_ROWS && T >= WIDE_TOKENS * B) prompt_attention<128, 8>(a, st);
+    else prompt_attention<128, 4>(a, st);
     return hipGetLastError();
 }
 
