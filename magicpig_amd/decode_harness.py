@@ -11,7 +11,11 @@ What runs where:
   * sparse layers : LSHSparseAttnServer.decode_full_fused -- q-hash + retrieve + sampled attention
                     (the hot path, HIP), static-window attention + LSE merge (HIP);
   * dense layers  : (0, 16, ...; models/attnserver.py:235-259) exact attention over the whole
-                    sequence = the dense mode of the same HIP kernel on a full-length store;
+                    sequence = the dense mode of the same HIP kernel on a full-length store, or
+                    (dense_cache="bf16" / "e4m3") attention over a paged cache;
+  * prompts       : `prefill` runs whole prompts, packed, through the layers (prompt_attention: HIP),
+                    `prefill_chunked` one long prompt piece by piece over a paged cache
+                    (PagedKVCache: HIP); both leave the attention state as `prefill_synthetic` does;
   * everything else (embedding, RMSNorm, q/k/v/o and MLP projections, RoPE, lm_head) is plain
     torch-ROCm -- model plumbing outside the north-star path, kept only so that an end-to-end
     tokens/s can be quoted next to the hot-path number.
@@ -32,6 +36,8 @@ import torch
 import torch.nn.functional as F
 
 from .attnserver import LSHSparseAttnServer
+from .paged_cache import PagedKVCache
+from .prompt_attention import prompt_attention
 from .sparse_attention import SparseAttentionServer
 
 
@@ -90,11 +96,15 @@ class SyntheticLlamaDecoder:
     def __init__(self, shape: LlamaShape = LLAMA_3_1_8B, K: int = 10, L: int = 150, batch_size: int = 1,
                  max_length: int = 8192, generation_buffer: int = 256, dense_layers=(0, 16, 32, 48, 64),
                  device: str = "cuda:0", dtype=torch.bfloat16, seed: int = 0,
-                 tp_rank: int = 0, tp_world: int = 1, tp_blocks: int | None = None, all_reduce=None):
+                 tp_rank: int = 0, tp_world: int = 1, tp_blocks: int | None = None, all_reduce=None,
+                 dense_cache: str = "store", page_size: int = 64):
         """tp_rank / tp_world: this process's slice of the heads and of the MLP (llama_dist.py); tp_blocks: the number of
         blocks the weights are DRAWN in (default tp_world; a TP = 1 decoder with tp_blocks = W holds the model of a TP = W
         run); all_reduce: callable summing a tensor over the ranks in place (default: torch.distributed when a process
-        group exists and tp_world > 1, else nothing to do)."""
+        group exists and tp_world > 1, else nothing to do).  dense_cache: the dense layers' keys and values in max_length
+        rows per request ("store") or in pages of page_size tokens, as they come ("bf16") or quantised ("e4m3")."""
+        if dense_cache not in ("store", "bf16", "e4m3"):
+            raise ValueError(f"dense_cache: expected 'store', 'bf16' or 'e4m3', got {dense_cache!r}")
         self.tp_rank, self.tp_world = tp_rank, tp_world
         self.tp_blocks = tp_blocks if tp_blocks is not None else tp_world
         assert 0 <= tp_rank < tp_world and self.tp_blocks % tp_world == 0
@@ -158,10 +168,20 @@ class SyntheticLlamaDecoder:
             max(1, len(self.sparse_layers)), H, Hkv, D, K=K, L=L, batch_size=batch_size,
             generation_buffer=generation_buffer, max_length=max_length, dense_layers=(), device=device,
             seed=seed + 7)
+        self.page_size = page_size
+        self.paged = dense_cache != "store"
         if self.dense_layers:
             with torch.cuda.device(self.device):
-                self.dense_server = SparseAttentionServer()
-                self.dense_server.alloc(len(self.dense_layers), H, Hkv, D, batch_size, max_length)
+                if self.paged:      # request b owns pages b * P .. (b + 1) * P
+                    pages = -(-max_length // page_size)
+                    self.dense_server = PagedKVCache()
+                    self.dense_server.alloc(len(self.dense_layers), H, Hkv, D, batch_size * pages, page_size,
+                                            kv_format=dense_cache)
+                    self.dense_table = torch.arange(batch_size * pages, device=self.device, dtype=torch.int32).view(batch_size, pages)
+                    self.step_rows = torch.arange(batch_size + 1, device=self.device, dtype=torch.int32)
+                else:
+                    self.dense_server = SparseAttentionServer()
+                    self.dense_server.alloc(len(self.dense_layers), H, Hkv, D, batch_size, max_length)
         BH = batch_size * H
         self.dense_len = torch.zeros((batch_size,), dtype=torch.int32, device=self.device)
         self.dense_nnz = torch.zeros((BH,), dtype=torch.int32, device=self.device)
@@ -184,21 +204,129 @@ class SyntheticLlamaDecoder:
                     ks.append(torch.randn((seq_len, 1, D), device=self.device, generator=g).to(self.dtype))
                     vs.append(torch.randn((seq_len, 1, D), device=self.device, generator=g).to(self.dtype))
                 k, v = torch.cat(ks, dim=1), torch.cat(vs, dim=1)
-            if layer in self.dense_index:
-                kk = k.transpose(0, 1).contiguous()
-                self.dense_server.fill(self.dense_index[layer], request_id, kk, v.transpose(0, 1).contiguous(),
-                                       kk.norm(p=2, dim=-1).float())
-            else:
-                li = self.sparse_index[layer]
-                self.attention_server.fill(li, request_id, k, v, seq_len)
-                self.attention_server.build_table(li, request_id, seq_len)
+            self._store_prompt(layer, request_id, k, v)
         self.dense_len[request_id] = seq_len
+
+    def _store_prompt(self, layer: int, request_id: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """One layer's keys and values of a whole prompt, bf16 [seq_len, Hkv, D], into the layer's attention state."""
+        n = k.shape[0]
+        if layer not in self.dense_index:
+            li = self.sparse_index[layer]
+            self.attention_server.fill(li, request_id, k, v, n)
+            self.attention_server.build_table(li, request_id, n)
+        elif self.paged:
+            rows, length = self._one_request(n, n)
+            self.dense_server.append(self.dense_index[layer], k, v, rows, self.dense_table[request_id:request_id + 1], length)
+        else:
+            kk = k.transpose(0, 1).contiguous()
+            self.dense_server.fill(self.dense_index[layer], request_id, kk, v.transpose(0, 1).contiguous(),
+                                   kk.norm(p=2, dim=-1).float())
+
+    def _one_request(self, new: int, length: int):
+        """(cu_seqlens, kv_len) of one request's `new` tokens, the last of `length`."""
+        t = torch.tensor([0, new, length], dtype=torch.int32).to(self.device)
+        return t[:2], t[2:]
+
+    # ------------------------------------------------------------------ prefill (the model's own)
+    def _prompt_layer(self, layer: int, hidden: torch.Tensor, position_ids: torch.Tensor, attend):
+        """models/llama.py:185-220 on packed prompt tokens: hidden [T, hidden_size], position_ids [T];
+        attend(q [T, H, D], k, v [T, Hkv, D]) -> [T, H, D]."""
+        W = self.layers[layer]
+        T, H, Hkv, D = hidden.shape[0], self.shape.num_attention_heads, self.shape.num_key_value_heads, self._head_dim
+        x = rms_norm(hidden, W["ln1"], self.shape.rms_norm_eps)
+        q = apply_rotary_pos_emb(F.linear(x, W["wq"]).view(T, H, D), self.cos_cache, self.sin_cache, position_ids)
+        k = apply_rotary_pos_emb(F.linear(x, W["wk"]).view(T, Hkv, D), self.cos_cache, self.sin_cache, position_ids)
+        v = F.linear(x, W["wv"]).view(T, Hkv, D)
+        o = F.linear(attend(q, k, v).reshape(T, H * D), W["wo"])
+        self._all_reduce(o)
+        h = hidden + o
+        y = rms_norm(h, W["ln2"], self.shape.rms_norm_eps)
+        y = F.linear(F.silu(F.linear(y, W["gate"])) * F.linear(y, W["up"]), W["down"])
+        self._all_reduce(y)
+        return h + y
+
+    def _check_prompt(self, request_id: int, n: int) -> None:
+        if not 0 <= request_id < self.batch_size:
+            raise ValueError(f"request_id {request_id}: the decoder holds {self.batch_size} requests")
+        least = 1
+        if self.sparse_layers:
+            least = self.attention_server.num_sink_tokens + self.attention_server.num_local_tokens + 1
+        if not least <= n <= self.max_length:
+            raise ValueError(f"prompt of request {request_id}: {n} tokens, expected {least} to {self.max_length}")
+
+    @torch.inference_mode()
+    def prefill(self, prompts, request_ids=None) -> torch.Tensor:
+        """`LLM.prefill` (models/llama.py:304-325) for several prompts at once: int64 token ids, 1-D, one tensor a request
+        (request_ids: which; default 0, 1, ...), packed one behind the other through every layer; each layer's keys and
+        values enter the attention state as `layer_prefill` does (:264, 282: fill + build_table).  Returns the logits of
+        each prompt's last token, f32 [prompts, vocab]."""
+        request_ids = list(range(len(prompts)) if request_ids is None else request_ids)
+        if not prompts or len(request_ids) != len(prompts) or len(set(request_ids)) != len(prompts):
+            raise ValueError("prefill: expected one request id per prompt, each once")
+        lens = [p.numel() for p in prompts]
+        for r, n in zip(request_ids, lens):
+            self._check_prompt(r, n)
+        ends = [sum(lens[:i]) for i in range(len(lens) + 1)]
+        cu = torch.tensor(ends, dtype=torch.int32).to(self.device)
+        pos = torch.cat([torch.arange(n, device=self.device) for n in lens])
+        hidden = F.embedding(torch.cat([p.reshape(-1).to(self.device) for p in prompts]), self.embed_tokens)
+
+        for layer in range(self.num_layers):
+            def attend(q, k, v):
+                out, _ = prompt_attention(q, k, v, cu)
+                for r, a, b in zip(request_ids, ends, ends[1:]):
+                    self._store_prompt(layer, r, k[a:b], v[a:b])
+                return out
+            hidden = self._prompt_layer(layer, hidden, pos, attend)
+        for r, n in zip(request_ids, lens):
+            self.dense_len[r] = n
+        last = rms_norm(hidden[cu[1:].long() - 1], self.norm_weight, self.shape.rms_norm_eps)
+        return F.linear(last, self.lm_head).float()
+
+    @torch.inference_mode()
+    def prefill_chunked(self, request_id: int, prompt: torch.Tensor, chunk: int = 2048, kv_format: str = "bf16") -> torch.Tensor:
+        """The same for one long prompt in pieces of `chunk` tokens, each through all layers before the next: activations of
+        one chunk instead of the whole prompt.  Meanwhile a paged cache of every layer holds the keys and values; at the end
+        they are read back into the attention state.  kv_format "e4m3" halves that cache: attention and state then see the
+        quantised rows.  Returns the logits of the last token, f32 [1, vocab]."""
+        n = prompt.numel()
+        self._check_prompt(request_id, n)
+        if chunk < 1:
+            raise ValueError("prefill_chunked: chunk must be at least 1")
+        pages = -(-n // self.page_size)
+        with torch.cuda.device(self.device):
+            cache = PagedKVCache()
+            cache.alloc(self.num_layers, self.shape.num_attention_heads, self.shape.num_key_value_heads, self._head_dim, pages,
+                        self.page_size, kv_format=kv_format)
+        table = torch.arange(pages, device=self.device, dtype=torch.int32).view(1, pages)
+        ids = prompt.reshape(-1).to(self.device)
+        for start in range(0, n, chunk):
+            end = min(n, start + chunk)
+            rows, length = self._one_request(end - start, end)
+            pos = torch.arange(start, end, device=self.device)
+            hidden = F.embedding(ids[start:end], self.embed_tokens)
+            for layer in range(self.num_layers):
+                def attend(q, k, v):
+                    cache.append(layer, k, v, rows, table, length)
+                    return cache.attention(layer, q, rows, table, length)[0]
+                hidden = self._prompt_layer(layer, hidden, pos, attend)
+        rows, length = self._one_request(n, n)
+        for layer in range(self.num_layers):
+            self._store_prompt(layer, request_id, *cache.read(layer, n, rows, table, length))
+        cache.check()                       # (waits for the stream: the cache may go)
+        self.dense_len[request_id] = n
+        last = rms_norm(hidden[-1:], self.norm_weight, self.shape.rms_norm_eps)
+        return F.linear(last, self.lm_head).float()
 
     # ------------------------------------------------------------------ decode
     def _dense_attention(self, q, k, v, layer: int) -> torch.Tensor:
         """models/attnserver.py:235-259: append, then exact attention over the whole sequence."""
         B, H, Hkv, D = self.batch_size, self.shape.num_attention_heads, self.shape.num_key_value_heads, self._head_dim
         di = self.dense_index[layer]
+        if self.paged:
+            self.dense_server.append(di, k.reshape(B, Hkv, D), v.reshape(B, Hkv, D), self.step_rows, self.dense_table, self.dense_len)
+            out, _ = self.dense_server.attention(di, q.reshape(B, H, D), self.step_rows, self.dense_table, self.dense_len)
+            return out.view(B, 1, H * D)
         self.dense_server.append(di, k.reshape(B, Hkv, D).contiguous(), v.reshape(B, Hkv, D).contiguous(),
                                  self.dense_len - 1)
         self.dense_server.full_attention(di, self.dense_out, self.dense_mve, q.reshape(B * H, D), self.dense_nnz)
