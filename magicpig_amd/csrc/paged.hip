@@ -196,9 +196,9 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(const CopyArgs a) {
 
 // ---------------------------------------------------------------- attention over the pages
 // Work.  Request b has ceil(n_b G / BM) tiles of rows and ceil(kv_b / TOK) tiles of keys.  A workgroup gets one tile of rows
-// of one kv head and at most `per` tiles of keys; per is the mean of what `units` workgroups a kv head would get, found by every
-// workgroup from the lengths on the device (so a captured graph follows them), at least MIN_KEYS tokens: short requests are
-// one part, long ones are cut into parts of one size, whatever the mix.  Parts of a row are joined by a second kernel.
+// of one kv head and one part of its keys.  What a part should be is found by every workgroup from the lengths on the device (so a
+// captured graph follows them): the work over `units` workgroups a kv head, at least MIN_KEYS tokens.  Short requests are
+// one part, long ones are cut evenly into parts of at most that, whatever the mix.  Parts of a row are joined by a second kernel.
 struct PagedAttnArgs {
     PagedRows r;
     const uint16_t* q;
@@ -215,48 +215,57 @@ struct PagedAttnArgs {
     int grid;                        // workgroups
 };
 
-constexpr int MIN_KEYS = 256;        // a part is at least this long: below, joining costs more than it spreads
+// Tokens of a part, at least: joining costs more than it spreads below.  One new token behind 2000 of one request takes 11.6 us
+// with parts of 256 and 13.8 with 512; behind 8000 12.4, and 14.2 with 128.  With 128 rows a workgroup there are more rows
+// to join: 512 new tokens of one request, 8 kv heads: 28.7 us in parts of 256, 18.7 in one.
+template <int BM>
+constexpr int MIN_KEYS = BM == 32 ? 256 : 512;
 
 struct PartOf {
     int seq;                         // -1: none
     int start, n, row0, kv;          // first row of q (token) and tokens of the request, first row of the tile, cached positions
-    int part, per;                   // which part, tiles of keys a part has
+    int part, parts;
 };
 
 template <int BM, int TOK>
 __device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units, int unit) {
     PartOf p;
     p.seq = -1;
-    p.start = p.n = p.row0 = p.kv = p.part = 0;
+    p.start = p.n = p.row0 = p.kv = p.part = p.parts = 0;
     auto first = [&](int i) { return min(max(r.cu[i], 0), r.T); };
     auto row_tiles = [&](int i) { return (max(first(i + 1) - first(i), 0) * G + BM - 1) / BM; };
     auto key_tiles = [&](int i) { return (int)(((int64_t)cached(r, r.kv_len[i]) + TOK - 1) / TOK); };
-    p.per = 0x7fffffff;
+    int per = 0x3fffffff;
     if (units > 0) {
-        float work = 0.f;            // (products of large counts; the quotient need not be exact)
+        float rows = 0.f, work = 0.f;           // (products of large counts; the quotient need not be exact)
         for (int base = 0; base < r.B; base += WAVE) {
             const int i = base + lane_id();
-            if (i < r.B) work += (float)row_tiles(i) * (float)key_tiles(i);
+            if (i >= r.B) continue;
+            const float rt = (float)row_tiles(i);
+            rows += rt;
+            work += rt * (float)key_tiles(i);
         }
-        p.per = max((int)__builtin_ceilf(fminf(wave_sum(work) / (float)units, 1e9f)), MIN_KEYS / TOK);
+        // half a part is lost to rounding up per tile of rows: aim so much lower that the parts still fit the chip at once
+        const float aim = fmaxf((float)units - 0.5f * wave_sum(rows), 0.5f * (float)units);
+        per = max((int)__builtin_ceilf(fminf(wave_sum(work) / aim, 1e9f)), MIN_KEYS<BM> / TOK);
     }
     int before = 0;
     for (int base = 0; base < r.B; base += WAVE) {
         const int i = base + lane_id();
-        const int rt = i < r.B ? row_tiles(i) : 0;
-        const int parts = rt > 0 ? max((key_tiles(i) + p.per - 1) / p.per, 1) : 0;
+        const int rt = i < r.B ? row_tiles(i) : 0, kt = rt > 0 ? key_tiles(i) : 0;
+        const int parts = rt == 0 ? 0 : 2 * (int64_t)kt < 3 * (int64_t)per ? 1 : (kt + per - 1) / per;      // (up to half longer before it is cut)
         const int sum = before + wave_incl_scan(rt * parts);
         const unsigned long long past = __ballot(sum > unit);
         if (past) {
             const int k = __ffsll(past) - 1;
-            const int np = __builtin_amdgcn_readlane(parts, k);
-            const int at = unit - (__builtin_amdgcn_readlane(sum, k) - __builtin_amdgcn_readlane(rt, k) * np);
+            p.parts = __builtin_amdgcn_readlane(parts, k);
+            const int at = unit - (__builtin_amdgcn_readlane(sum, k) - __builtin_amdgcn_readlane(rt, k) * p.parts);
             p.seq = base + k;
             p.start = first(p.seq);
             p.n = first(p.seq + 1) - p.start;
             p.kv = cached(r, r.kv_len[p.seq]);
-            p.row0 = at / np * BM;
-            p.part = at % np;
+            p.row0 = at / p.parts * BM;
+            p.part = at % p.parts;
             return p;
         }
         before = __builtin_amdgcn_readlane(sum, WAVE - 1);
@@ -279,9 +288,9 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttn
     const int rows = t.n * a.G, old = t.kv - t.n;                     // old: positions in front of the new tokens
     const int lim_lo = old + t.row0 / a.G, lim_hi = old + min(t.row0 + BM - 1, rows - 1) / a.G;
     const int all = lim_hi < 0 ? 0 : lim_hi / TILE_TOKENS + 1;
-    const int used = all > t.per ? (all + t.per - 1) / t.per : 1;
+    const int used = max(min(t.parts, all), 1);
     if (t.part >= used) return;
-    const int begin = t.part * min(t.per, all), end = min(all, begin + min(t.per, all));
+    const int begin = (int)((int64_t)all * t.part / used), end = (int)((int64_t)all * (t.part + 1) / used);
 
     const int wrow = t.row0 + 32 * w;
     const int row = min(wrow + (l & 31), rows - 1);
@@ -394,9 +403,9 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(const PagedAttnArgs 
     const int rows = t.n * a.G, old = t.kv - t.n;
     const int lim_lo = old + t.row0 / a.G, lim_hi = old + min(t.row0 + BM - 1, rows - 1) / a.G;
     const int all = lim_hi < 0 ? 0 : lim_hi / TOK + 1;
-    const int used = all > t.per ? (all + t.per - 1) / t.per : 1;
+    const int used = max(min(t.parts, all), 1);
     if (t.part >= used) return;
-    const int begin = t.part * min(t.per, all), end = min(all, begin + min(t.per, all));
+    const int begin = (int)((int64_t)all * t.part / used), end = (int)((int64_t)all * (t.part + 1) / used);
     const int whole = min(lim_lo < 0 ? 0 : (lim_lo + 1) / TOK, end);
 
     RowState<D> st;
@@ -423,8 +432,8 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(const PagedAttnArgs 
             const int r = (i * 64 + l) / PER_ROW, p = (i * 64 + l) % PER_ROW;
             const uint64_t x = (uint32_t)__builtin_amdgcn_ds_bpermute(r * 4, (int)at);
             const char* src = a.pool + x * (E4M3 ? 2 * D : 4 * D) + p * 16;
-            kr[i] = *reinterpret_cast<const u32x4*>(src);
-            vr[i] = *reinterpret_cast<const u32x4*>(src + (E4M3 ? D : 2 * D));
+            kr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src));
+            vr[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + (E4M3 ? D : 2 * D)));
             if (E4M3) sr[i] = *reinterpret_cast<const uint16_t*>(a.scale + x * 2);
         }
     };
@@ -529,45 +538,83 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(const PagedAttnArgs 
 }
 
 // Parts of a row joined: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, in an order that does not depend on when they
-// were ready.  A workgroup a row, its waves take the parts in turn.
-template <int D, int BM>
+// were ready.  WAVES waves a row take its parts in turn, four at a time, each with a running maximum of its own: nothing is
+// waited for but the row's place, then the parts.
+template <int D, int BM, int WAVES>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
-    constexpr int W = D / 64;
-    __shared__ float so[4][D], sl[4];
-    const int64_t row = blockIdx.x;
-    const int tok = (int)(row / a.H), l = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (tok < a.r.cu[0] || tok >= a.r.cu[a.r.B]) return;              // (part_of of such a row was never written)
-    const int2 of = a.part_of[row];
-    const int n = of.y;
+    constexpr int W = D / 64, ROWS = 4 / WAVES;
+    __shared__ float so[4][D];
+    __shared__ float2 sml[4];
+    const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = (int64_t)blockIdx.x * ROWS + w / WAVES;
+    const int tok = (int)(row / a.H), lo = a.r.cu[0], hi = a.r.cu[a.r.B];
+    const int2 of = tok < a.r.T ? a.part_of[row] : make_int2(0, 0);
+    // (part_of of a row outside the requests was never written, and offsets that are none could leave anything)
     const int64_t at = of.x, step = (int64_t)a.r.Hkv * BM;            // the parts of a row are neighbours among its head's workgroups
-    if (n <= 1 || at < 0 || at + (n - 1) * step >= (int64_t)a.grid * BM) return;     // (offsets that are none could leave anything)
-    float m = NEG_INF;
-    for (int s = l; s < n; s += WAVE) m = fmaxf(m, a.part_ml[at + s * step].x);
-    m = wave_max(m);
-    const float off = m == NEG_INF ? 0.f : m;
-    float sum = 0.f, o[W];
+    const bool mine = tok >= lo && tok < hi && of.y > 1 && at >= 0 && at + (of.y - 1) * step < (int64_t)a.grid * BM;
+    const int n = mine ? of.y : 0;
+    if (WAVES == 4 && n == 0) return;
+    float m = NEG_INF, sum = 0.f, o[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) o[i] = 0.f;
-#pragma unroll 4
-    for (int s = w; s < n; s += 4) {
-        const float2 x = a.part_ml[at + s * step];
-        const float* po = a.part_o + (at + s * step) * D + l * W;
-        const float wt = __builtin_amdgcn_exp2f(x.x - off);
-        sum += wt * x.y;
+    for (int s0 = w % WAVES; s0 < n; s0 += 4 * WAVES) {
+        float2 x[4];
+        float y[4][W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) o[i] += wt * po[i];
+        for (int u = 0; u < 4; ++u) {
+            const int64_t part = at + min(s0 + u * WAVES, n - 1) * step;
+            x[u] = a.part_ml[part];
+#pragma unroll
+            for (int i = 0; i < W; ++i) y[u][i] = a.part_o[part * D + l * W + i];
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (s0 + u * WAVES >= n) x[u] = make_float2(NEG_INF, 0.f);
+            top = fmaxf(top, x[u].x);
+        }
+        const float off = top == NEG_INF ? 0.f : top, f = __builtin_amdgcn_exp2f(m - off);
+        m = top;
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] *= f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float wt = __builtin_amdgcn_exp2f(x[u].x - off);
+            sum += wt * x[u].y;
+#pragma unroll
+            for (int i = 0; i < W; ++i) o[i] += s0 + u * WAVES < n ? wt * y[u][i] : 0.f;
+        }
     }
+    if (WAVES == 4) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) so[w][l * W + i] = o[i];
-    if (l == 0) sl[w] = sum;
-    __syncthreads();
-    if (threadIdx.x >= D / 2) return;
-    const float total = (sl[0] + sl[1]) + (sl[2] + sl[3]), inv = total == 0.f ? 0.f : 1.f / total;
-    const int d = 2 * threadIdx.x;
-    const float x = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
-    const float y = (so[0][d + 1] + so[1][d + 1]) + (so[2][d + 1] + so[3][d + 1]);
-    *reinterpret_cast<uint32_t*>(a.out + row * D + d) = pack_bf16(x * inv, y * inv);
-    if (a.lse != nullptr && threadIdx.x == 0) a.lse[row] = log_sum(m, total);
+        for (int i = 0; i < W; ++i) so[w][l * W + i] = o[i];
+        if (l == 0) sml[w] = make_float2(m, sum);
+        __syncthreads();
+        if (w > 0) return;
+        float2 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x[k] = sml[k];
+            m = fmaxf(m, x[k].x);
+        }
+        const float off = m == NEG_INF ? 0.f : m;
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float wt = __builtin_amdgcn_exp2f(x[k].x - off);
+            sum += wt * x[k].y;
+#pragma unroll
+            for (int i = 0; i < W; ++i) o[i] += wt * so[k][l * W + i];
+        }
+    }
+    if (n == 0) return;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (W == 2) *reinterpret_cast<uint32_t*>(a.out + row * D + 2 * l) = pack_bf16(o[0] * inv, o[W - 1] * inv);
+    else a.out[row * D + l] = (uint16_t)(pack_bf16(o[0] * inv, 0.f) & 0xffffu);
+    if (a.lse != nullptr && l == 0) a.lse[row] = log_sum(m, sum);
 }
 
 // ---------------------------------------------------------------- host
@@ -630,7 +677,7 @@ PagedPlan paged_plan(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, 
     const int BM = p.step ? 32 : 128;
     const int64_t tiles = T * G / BM + live, target = 2 * (int64_t)cus;           // two workgroups a CU
     // rows alone that give every CU eight workgroups are not cut further; neither is what fits one part
-    p.units = tiles * Hkv >= 4 * target || capacity <= MIN_KEYS ? 0 : (int)((target + Hkv - 1) / Hkv);
+    p.units = tiles * Hkv >= 4 * target || capacity <= (p.step ? MIN_KEYS<32> : MIN_KEYS<128>) ? 0 : (int)((target + Hkv - 1) / Hkv);
     p.grid = (tiles + p.units + (p.units > 0)) * Hkv;
     p.bytes = p.units > 0 ? p.grid * BM * ((int64_t)D * 4 + 8) + T * H * 8 : 0;
     return p;
@@ -638,13 +685,14 @@ PagedPlan paged_plan(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, 
 
 template <int D, bool E4M3>
 static void paged_attention(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
-    const dim3 grid((unsigned)p.grid), join((unsigned)(a.r.T * a.H));
+    const int64_t rows = (int64_t)a.r.T * a.H;
+    const dim3 grid((unsigned)p.grid);
     if (p.step) {
         paged_step_kernel<D, E4M3><<<grid, 256, 0, st>>>(a);
-        if (p.units > 0) paged_join_kernel<D, 32><<<join, 256, 0, st>>>(a);
+        if (p.units > 0) paged_join_kernel<D, 32, 4><<<dim3((unsigned)rows), 256, 0, st>>>(a);        // few rows, many parts
     } else {
         paged_attention_kernel<D, E4M3><<<grid, 256, 0, st>>>(a);
-        if (p.units > 0) paged_join_kernel<D, 128><<<join, 256, 0, st>>>(a);
+        if (p.units > 0) paged_join_kernel<D, 128, 1><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(a);
     }
 }
 
