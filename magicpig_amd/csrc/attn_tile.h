@@ -316,4 +316,60 @@ __device__ __forceinline__ void store_rows(const RowState<D>& st, uint16_t* out,
     if (lse != nullptr && h == 0) *lse = log_sum(st.m, l);
 }
 
+// Four waves that folded different keys into the same 32 rows: their sums joined.  Wave w leaves its 32 rows, f32, in its own
+// 32 D * 4 bytes of LDS (`mine`; the waves' blocks lie `apart` 16-byte chunks from each other at `all`), chunk c of row r at place
+// c ^ r, as a column's rows would all lie in one bank otherwise.  Then 8 threads a row: thread i gets chunks (i % 8) D / 32
+// .. of row i / 8, scaled to the maximum m, and the row's sum of weights.  One barrier; all 256 threads call it.
+template <int D>
+__device__ __forceinline__ void join_waves(const RowState<D>& st, f32x4* mine, const f32x4* all, int apart, float2 (&ml)[4][32],
+                                           float& m, float& total, f32x4 (&o)[D / 32]) {
+    constexpr int NC = D / 4;                            // chunks of a row
+    const int l = lane_id(), w = threadIdx.x >> 6;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // (the block held the wave's tile: its last reads come first)
+    const float sum = halves_sum(st.l);
+    if (l < 32) ml[w][l] = make_float2(st.m, sum);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            mine[(l & 31) * NC + ((8 * i + 2 * g + (l >> 5)) ^ (l & (NC - 1) & 31))] =
+                f32x4{st.o[i][4 * g], st.o[i][4 * g + 1], st.o[i][4 * g + 2], st.o[i][4 * g + 3]};
+    __syncthreads();
+    const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (NC / 8);
+    float2 x[4];
+    m = NEG_INF;
+    total = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        x[k] = ml[k][r];
+        m = fmaxf(m, x[k].x);
+    }
+    const float off = m == NEG_INF ? 0.f : m;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float wt = __builtin_amdgcn_exp2f(x[k].x - off);
+        total += wt * x[k].y;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            const f32x4 y = all[k * apart + r * NC + ((c0 + c) ^ (r & (NC - 1)))];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c][e] += wt * y[e];
+        }
+    }
+}
+// ... and as they leave: this thread's chunks of its row
+template <int D>
+__device__ __forceinline__ void store_chunks(uint16_t* out, const f32x4 (&o)[D / 32], float total) {
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+        u32x2 b;
+        b[0] = pack_bf16(o[c][0] * inv, o[c][1] * inv);
+        b[1] = pack_bf16(o[c][2] * inv, o[c][3] * inv);
+        *reinterpret_cast<u32x2*>(out + 4 * ((threadIdx.x & 7) * (D / 32) + c)) = b;
+    }
+}
+
 }  // namespace mp

@@ -391,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttn
 // e4m3, eight waves a CU) are in flight while the tile before it is folded in.
 template <int D, bool E4M3>
 __global__ __launch_bounds__(256, 2) void paged_step_kernel(const PagedAttnArgs a) {
-    constexpr int BM = 32, TOK = 32, KB = TOK * 2 * D, NC = D / 4;     // NC: 16-byte chunks of an f32 row
+    constexpr int BM = 32, TOK = 32, KB = TOK * 2 * D;
     constexpr int PER_ROW = E4M3 ? D / 16 : D / 8;
     constexpr int PASSES = TOK * PER_ROW / 64;
     __shared__ __attribute__((aligned(1024))) char lds[4][2 * KB];     // a wave's K and V tile; at the end its 32 rows of sums
@@ -424,8 +424,6 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(const PagedAttnArgs 
     auto fetch_pages = [&](int tile) { page = table[position(tile) >> a.r.shift]; };
     auto load = [&](int tile) {
         const int pg = max(page_ok(a.r, page), 0);
-        int l = lane_id();
-        asm volatile("" : "+v"(l));          // (the few things below that depend on it are not worth registers of their own)
         const uint32_t at = (((uint32_t)pg * (uint32_t)a.r.Hkv + (uint32_t)head) << a.r.shift) | (uint32_t)(position(tile) & slot_mask);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
@@ -465,73 +463,35 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(const PagedAttnArgs 
         load(j);
         if (j + 4 < end) fetch_pages(j + 4);
     }
-    auto ahead = [&] {
+    for (; j < whole; j += 4) {
+        store();
+        __builtin_amdgcn_sched_barrier(0);           // the next tile's loads take the registers just stored
         if (j + 4 < end) {
             load(j + 4);
             if (j + 8 < end) fetch_pages(j + 8);
         }
-    };
-    for (; j < whole; j += 4) {
-        store();
-        __builtin_amdgcn_sched_barrier(0);           // the next tile's loads take the registers just stored
-        ahead();
         fold_tile<D, 1, false>(st, kt, vt, a.c, 0);
     }
-    for (; j < end; j += 4) {            // the last tile or two: nothing to load beside it, or little
+    if (j < end) {                       // 32 rows end in at most two tiles: one a wave
         store();
         fold_tile<D, 1, true>(st, kt, vt, a.c, lim - j * TOK);
-        ahead();
     }
 
-    // the four waves' sums, f32, row after row with chunks permuted (the rows of a column lie in one bank otherwise)
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const float sum = halves_sum(st.l);
-    if (l < 32) ml[w][l] = make_float2(st.m, sum);
-    f32x4* mine = reinterpret_cast<f32x4*>(lds[w]) + (l & 31) * NC;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-            mine[(8 * i + 2 * g + (l >> 5)) ^ (l & (NC - 1) & 31)] =
-                f32x4{st.o[i][4 * g], st.o[i][4 * g + 1], st.o[i][4 * g + 2], st.o[i][4 * g + 3]};
-    __syncthreads();
-    const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * (NC / 8), grow = t.row0 + r;     // 8 threads a row
+    float m, total;
+    f32x4 o[D / 32];
+    const int r = threadIdx.x >> 3, grow = t.row0 + r;
+    join_waves<D>(st, reinterpret_cast<f32x4*>(lds[w]), reinterpret_cast<const f32x4*>(lds[0]), 2 * KB / 16, ml, m, total, o);
     if (grow >= rows) return;
-    float2 x[4];
-    float m = NEG_INF, wt[4], total = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        x[k] = ml[k][r];
-        m = fmaxf(m, x[k].x);
-    }
-    const float off = m == NEG_INF ? 0.f : m;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        wt[k] = __builtin_amdgcn_exp2f(x[k].x - off);
-        total += wt[k] * x[k].y;
-    }
     const int64_t orow = (int64_t)(t.start + grow / a.G) * a.H + head * a.G + grow % a.G;
     const int64_t prow = (int64_t)blockIdx.x * BM + r;
-    const float inv = used > 1 ? 1.f : total == 0.f ? 0.f : 1.f / total;
+    if (used > 1) {
 #pragma unroll
-    for (int c = 0; c < NC / 8; ++c) {
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const f32x4 y = reinterpret_cast<const f32x4*>(lds[k])[r * NC + ((c0 + c) ^ (r & (NC - 1) & 31))];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] += wt[k] * y[e];
-        }
-        if (used > 1) {
-            *reinterpret_cast<f32x4*>(a.part_o + prow * D + 4 * (c0 + c)) = o;
-        } else {
-            u32x2 b;
-            b[0] = pack_bf16(o[0] * inv, o[1] * inv);
-            b[1] = pack_bf16(o[2] * inv, o[3] * inv);
-            *reinterpret_cast<u32x2*>(a.out + orow * D + 4 * (c0 + c)) = b;
-        }
+        for (int c = 0; c < D / 32; ++c)
+            *reinterpret_cast<f32x4*>(a.part_o + prow * D + 4 * ((threadIdx.x & 7) * (D / 32) + c)) = o[c];
+    } else {
+        store_chunks<D>(a.out + orow * D, o, total);
     }
-    if (c0 != 0) return;
+    if ((threadIdx.x & 7) != 0) return;
     if (a.units > 0 && t.part == 0) a.part_of[orow] = make_int2((int)blockIdx.x * BM + r, used);
     if (used > 1) a.part_ml[prow] = make_float2(m, total);
     else if (a.lse != nullptr) a.lse[orow] = log_sum(m, total);
@@ -672,8 +632,11 @@ struct PagedPlan {
 PagedPlan paged_plan(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus) {
     const int64_t G = H / Hkv, live = T < B ? T : B;
     PagedPlan p;
-    // by the mean rows of a request and kv head: up to one tile of 32 the keys are read once either way
-    p.step = T * G <= 32 * live;
+    // Up to 32 rows a request and kv head on average, the keys are read once either way.  Beyond, every tile of 32 rows reads
+    // them again, which costs less than the few, long workgroups of 128 rows as long as it is little in all: 16 new tokens of one
+    // request, 32 heads over 8, behind 2000 tokens: 12.8 us against 19.8; behind 8000 (2^17 tokens x tiles) 21.4 against
+    // 24.4; behind 32 000 50 against 42; 8 such requests behind 2000 (2^18) 31 against 26.  (The host knows the tables' size, not the lengths.)
+    p.step = T * G <= 32 * live || (T * G + 31) / 32 * Hkv * capacity <= 1 << 17;
     const int BM = p.step ? 32 : 128;
     const int64_t tiles = T * G / BM + live, target = 2 * (int64_t)cus;           // two workgroups a CU
     // rows alone that give every CU eight workgroups are not cut further; neither is what fits one part

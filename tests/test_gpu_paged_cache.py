@@ -171,6 +171,32 @@ def test_attention_against_64_bits(page, pairs, H, Hkv, D, fmt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("pairs,H,Hkv", [
+    ([(40, 20000)], 32, 8), ([(300, 6000), (1, 9), (77, 5000)], 16, 4), ([(1500, 1500)], 32, 8), ([(5000, 5000), (300, 200)], 32, 8)])
+def test_workgroups_of_many_rows_whole_and_in_parts(pairs, H, Hkv, D, fmt):
+    s = Setup(pairs, 64, H, Hkv, D, fmt, seed=21).fill()
+    s.compare(*s.attend())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pairs,H,Hkv", [([(30, 100), (1, 600)], 8, 2), ([(300, 4000), (1, 600)], 32, 8)], ids=["few rows", "many rows"])
+def test_nonfinite_values_in_every_kernel(pairs, H, Hkv):
+    s = Setup(pairs, 16, H, Hkv, 128, "bf16", seed=22)
+    s.v[0][-1, 0, 3] = float("inf")
+    s.v[0][-2, 1, 4] = float("nan")
+    s.v[0][-20, 0, 5] = float("-inf")
+    s.v[1][-1, 1] = float("-inf")
+    s.k[0][-3, Hkv - 1, 7] = float("nan")
+    s.fill()
+    pages = s.cache.get_pages(0)[0]
+    for b, (n, kv) in enumerate(pairs):
+        pages[int(s.table[b, (kv - 1) // 16]), :, (kv - 1) % 16 + 1:] = float("nan")
+    s.compare(*s.attend())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 def test_long_cache_in_many_parts(fmt):
     s = Setup([(1, 40000), (2, 17), (1, 9000)], 64, 8, 2, 128, fmt, seed=11).fill()
     s.compare(*s.attend(scale=0.2), scale=0.2)

@@ -65,6 +65,42 @@ def test_rows_outside_the_sequences_stay():
         assert bool((out[a:b] == 7.0).all()) and bool((lse[a:b] == -3.0).all())
 
 
+# few rows; more than 2^14; more than 2^17 of long sequences: workgroups of 32, 128 and 256 rows
+SIZES = [([70, 3, 200], 8, 2), ([400, 3, 300], 32, 4), ([2100, 2300], 32, 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,Hkv", SIZES, ids=["32", "128", "256"])
+def test_every_kernel_on_slices_outside_rows_and_nonfinite_tokens(lens, H, Hkv, D):
+    q, k, v, cu = packed(lens, H, Hkv, D, seed=31, before=2, behind=3)
+    ends = cu.tolist()
+    v[ends[1] - 1, 0, 1] = float("inf")                    # the last token of the first sequence
+    v[ends[1] - 2, Hkv - 1, D - 1] = float("nan")
+    v[ends[-2] + 40, 0] = float("-inf")                    # the 41st of the last
+    k[ends[-1] - 1, Hkv - 1, 0] = float("nan")
+    q[0] = k[1] = v[-1] = k[-2] = float("nan")             # rows of no sequence
+    qkv = torch.cat([q, k, v], dim=1)
+    out, lse = torch.full_like(q, 7.0), torch.full((q.shape[0], H), -3.0, device="cuda")
+    mp.prompt_attention(qkv[:, :H], qkv[:, H:H + Hkv], qkv[:, H + Hkv:], cu, out=out, lse=lse)
+    compare(q, k, v, cu, out, lse)
+    assert bool(torch.isfinite(out[ends[0]:ends[1] - 2]).all()) and bool(torch.isfinite(out[ends[-2]:ends[-2] + 40]).all())
+    for a, b in ((0, ends[0]), (ends[-1], q.shape[0])):
+        assert bool((out[a:b] == 7.0).all()) and bool((lse[a:b] == -3.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,Hkv", SIZES, ids=["32", "128", "256"])
+def test_every_kernel_on_growing_and_falling_logits(lens, H, Hkv, D):
+    """Logits that climb by thousands along the keys (the running maximum has to follow again and again) and fall back."""
+    q, k, v, cu = packed(lens, H, Hkv, D, seed=32)
+    ramp = torch.linspace(0, 30, q.shape[0], device="cuda")[:, None, None]
+    for ks in (k * ramp, k * ramp.flip(0)):
+        ks = (ks + q[:, :Hkv] * ramp).bfloat16()
+        compare(q, ks, v, cu, *mp.prompt_attention(q, ks, v, cu))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
