@@ -39,6 +39,12 @@ __device__ __forceinline__ int page_ok(const PagedRows& r, int page) {
     return -1;
 }
 
+// row of the cache that holds position `pos` (in page `page`, or page 0 if there is no such page) of a kv head
+__device__ __forceinline__ uint32_t cache_row(const PagedRows& r, int page, int head, int pos) {
+    const uint32_t pg = (uint32_t)max(page_ok(r, page), 0);
+    return ((pg * (uint32_t)r.Hkv + (uint32_t)head) << r.shift) | (uint32_t)(pos & ((1 << r.shift) - 1));
+}
+
 // e4m3 pairs -> bf16 pairs times a power of two
 __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float s) {
     u32x4 w;
@@ -221,6 +227,11 @@ struct PagedAttnArgs {
 template <int BM>
 constexpr int MIN_KEYS = BM == 32 ? 256 : 512;
 
+// From here on 256 rows a workgroup at head_dim 128, which read the keys from L2 half as often: 4096 new tokens of 32 heads over 8
+// behind 32 000 1.99 ms against 2.12, 16 x 512 of 8 heads over 1 behind 2000 (e4m3) 82 us against 88; at the border itself it is
+// even (2048 of 32 heads behind 32 000 1.05 ms against 1.11, behind 67 584 2.33 against 2.30).
+constexpr int64_t WIDE_ROWS = 1 << 16;
+
 struct PartOf {
     int seq;                         // -1: none
     int start, n, row0, kv;          // first row of q (token) and tokens of the request, first row of the tile, cached positions
@@ -253,7 +264,8 @@ __device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units
     for (int base = 0; base < r.B; base += WAVE) {
         const int i = base + lane_id();
         const int rt = i < r.B ? row_tiles(i) : 0, kt = rt > 0 ? key_tiles(i) : 0;
-        const int parts = rt == 0 ? 0 : 2 * (int64_t)kt < 3 * (int64_t)per ? 1 : (kt + per - 1) / per;      // (up to half longer before it is cut)
+        // (what is less than half longer than the least part is not cut)
+        const int parts = rt == 0 ? 0 : 2 * kt < 3 * (MIN_KEYS<BM> / TOK) ? 1 : (kt + per - 1) / per;
         const int sum = before + wave_incl_scan(rt * parts);
         const unsigned long long past = __ballot(sum > unit);
         if (past) {
@@ -273,13 +285,13 @@ __device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units
     return p;
 }
 
-// Many rows: 128 of one (request, kv head) a workgroup, everything else as in prompt.hip.  An e4m3 tile passes through
+// Many rows: 128 or 256 of one (request, kv head) a workgroup, everything else as in prompt.hip.  An e4m3 tile passes through
 // registers on its way to LDS: loaded while the tile before it is folded in, widened behind it (exact).
-template <int D, bool E4M3>
-__global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttnArgs a) {
-    constexpr int BM = 128, CPR = D / 8, KB = TILE_TOKENS * 2 * D;
+template <int D, bool E4M3, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(const PagedAttnArgs a) {
+    constexpr int THREADS = 64 * WAVES, BM = 32 * WAVES, CPR = D / 8, KB = TILE_TOKENS * 2 * D;
     constexpr int PER_ROW = E4M3 ? CPR / 2 : CPR;                     // 16-byte pieces of a cached row
-    constexpr int PASSES = TILE_TOKENS * PER_ROW / 256;
+    constexpr int PASSES = TILE_TOKENS * PER_ROW / THREADS;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][KB];
     const int head = blockIdx.x % a.r.Hkv;
     const PartOf t = find_part<BM, TILE_TOKENS>(a.r, a.G, a.units, (int)(blockIdx.x / a.r.Hkv));
@@ -302,22 +314,19 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttn
     const int seen = wrow < rows && wave_hi >= 0 ? min(wave_hi / TILE_TOKENS + 1, end) : 0;
 
     const int32_t* table = a.r.table + (int64_t)t.seq * a.r.P;
-    const int slot_mask = (1 << a.r.shift) - 1;
-    int page[PASSES];
+    // lane l looks up the cache row of token l of a tile (positions behind the last visible one: that one again, masked);
+    // the lanes that load a row get it from there.  (A row number fits 32 bits: 2^32 rows are more than any HBM.)
+    int page = 0;
     u32x4 kr[PASSES], vr[PASSES];
     uint32_t sr[PASSES];
-    // positions behind the last visible one: that one again, masked
-    auto position = [&](int tile, int i) { return min(tile * TILE_TOKENS + (i * 256 + (int)threadIdx.x) / PER_ROW, lim_hi); };
-    auto fetch_pages = [&](int tile) {
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) page[i] = table[position(tile, i) >> a.r.shift];
-    };
+    auto position = [&](int tile) { return min(tile * TILE_TOKENS + l, lim_hi); };
+    auto fetch_pages = [&](int tile) { page = table[position(tile) >> a.r.shift]; };
     auto stage = [&](int tile) {
+        const uint32_t row_of = cache_row(a.r, page, head, position(tile));
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            const int idx = i * 256 + (int)threadIdx.x, r = idx / PER_ROW, p = idx % PER_ROW;
-            const int pg = max(page_ok(a.r, page[i]), 0);
-            const int64_t at = (((int64_t)pg * a.r.Hkv + head) << a.r.shift) | (position(tile, i) & slot_mask);
+            const int idx = i * THREADS + (int)threadIdx.x, r = idx / PER_ROW, p = idx % PER_ROW;
+            const uint64_t at = (uint32_t)__builtin_amdgcn_ds_bpermute(r * 4, (int)row_of);
             if (E4M3) {
                 const char* src = a.pool + at * (2 * D) + p * 16;
                 kr[i] = *reinterpret_cast<const u32x4*>(src);
@@ -325,7 +334,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttn
                 sr[i] = *reinterpret_cast<const uint16_t*>(a.scale + at * 2);
             } else {
                 const char* src = a.pool + at * (4 * D);
-                char* dst = lds[tile & 1][0] + (i * 256 + w * 64) * 16;
+                char* dst = lds[tile & 1][0] + (i * THREADS + w * 64) * 16;
                 dma16(src + ((p ^ key_swizzle<D>(r)) << 4), dst);
                 dma16(src + 2 * D + ((p ^ value_swizzle<D>(r)) << 4), dst + KB);
             }
@@ -335,7 +344,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_kernel(const PagedAttn
         if (!E4M3) return;
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-            const int idx = i * 256 + (int)threadIdx.x, r = idx / PER_ROW, p = idx % PER_ROW;
+            const int idx = i * THREADS + (int)threadIdx.x, r = idx / PER_ROW, p = idx % PER_ROW;
             char* kt = lds[tile & 1][0] + r * 2 * D;
             const float ks = __uint_as_float((sr[i] & 255u) << 23), vs = __uint_as_float((sr[i] >> 8) << 23);
 #pragma unroll
@@ -413,18 +422,14 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(const PagedAttnArgs 
     load_rows<D>(st, a.q + (int64_t)(t.start + tok) * a.q_st + (int64_t)(head * a.G + row % a.G) * a.q_sh);
 
     const int32_t* table = a.r.table + (int64_t)t.seq * a.r.P;
-    const int slot_mask = (1 << a.r.shift) - 1;
     char *kt = lds[w], *vt = lds[w] + KB;
-    // lane l looks up the cache row of token l % 32 of a tile (positions behind the last visible one: that one again,
-    // masked); the lanes that load a row get it from there.  (A row number fits 32 bits: 2^32 rows are more than any HBM.)
-    int page = 0;
+    int page = 0;                        // as above; lane l: token l % 32
     u32x4 kr[PASSES], vr[PASSES];
     uint32_t sr[PASSES];
     auto position = [&](int tile) { return min(tile * TOK + (l & 31), lim_hi); };
     auto fetch_pages = [&](int tile) { page = table[position(tile) >> a.r.shift]; };
     auto load = [&](int tile) {
-        const int pg = max(page_ok(a.r, page), 0);
-        const uint32_t at = (((uint32_t)pg * (uint32_t)a.r.Hkv + (uint32_t)head) << a.r.shift) | (uint32_t)(position(tile) & slot_mask);
+        const uint32_t at = cache_row(a.r, page, head, position(tile));
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int r = (i * 64 + l) / PER_ROW, p = (i * 64 + l) % PER_ROW;
@@ -624,7 +629,7 @@ hipError_t launch_paged_read(uint16_t* k, uint16_t* v, const int32_t* cu, int B,
 
 // How attention cuts a call's work, from what the host knows.
 struct PagedPlan {
-    bool step;           // 32 rows a workgroup (few rows a request) instead of 128
+    int rows;            // of a workgroup: 32 (few rows a request), 128 or 256
     int units;           // workgroups a kv head that the keys are cut for, 0 = not cut
     int64_t grid;        // workgroups, at most
     int64_t bytes;       // workspace
@@ -636,26 +641,31 @@ PagedPlan paged_plan(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, 
     // them again, which costs less than the few, long workgroups of 128 rows as long as it is little in all: 16 new tokens of one
     // request, 32 heads over 8, behind 2000 tokens: 12.8 us against 19.8; behind 8000 (2^17 tokens x tiles) 21.4 against
     // 24.4; behind 32 000 50 against 42; 8 such requests behind 2000 (2^18) 31 against 26.  (The host knows the tables' size, not the lengths.)
-    p.step = T * G <= 32 * live || (T * G + 31) / 32 * Hkv * capacity <= 1 << 17;
-    const int BM = p.step ? 32 : 128;
-    const int64_t tiles = T * G / BM + live, target = 2 * (int64_t)cus;           // two workgroups a CU
+    const bool step = T * G <= 32 * live || (T * G + 31) / 32 * Hkv * capacity <= 1 << 17;
+    p.rows = step ? 32 : D == 128 && T * H >= WIDE_ROWS ? 256 : 128;
+    const int64_t tiles = T * G / p.rows + live, target = (p.rows == 256 ? 1 : 2) * (int64_t)cus;        // workgroups that fit the chip
     // rows alone that give every CU eight workgroups are not cut further; neither is what fits one part
-    p.units = tiles * Hkv >= 4 * target || capacity <= (p.step ? MIN_KEYS<32> : MIN_KEYS<128>) ? 0 : (int)((target + Hkv - 1) / Hkv);
+    p.units = tiles * Hkv >= 4 * target || capacity <= (step ? MIN_KEYS<32> : MIN_KEYS<128>) ? 0 : (int)((target + Hkv - 1) / Hkv);
     p.grid = (tiles + p.units + (p.units > 0)) * Hkv;
-    p.bytes = p.units > 0 ? p.grid * BM * ((int64_t)D * 4 + 8) + T * H * 8 : 0;
+    p.bytes = p.units > 0 ? p.grid * p.rows * ((int64_t)D * 4 + 8) + T * H * 8 : 0;
     return p;
 }
 
 template <int D, bool E4M3>
 static void paged_attention(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
     const int64_t rows = (int64_t)a.r.T * a.H;
-    const dim3 grid((unsigned)p.grid);
-    if (p.step) {
+    const dim3 grid((unsigned)p.grid), join((unsigned)((rows + 3) / 4));
+    if (p.rows == 32) {
         paged_step_kernel<D, E4M3><<<grid, 256, 0, st>>>(a);
         if (p.units > 0) paged_join_kernel<D, 32, 4><<<dim3((unsigned)rows), 256, 0, st>>>(a);        // few rows, many parts
+    } else if (p.rows == 256) {
+        if constexpr (D == 128) {
+            paged_attention_kernel<D, E4M3, 8><<<grid, 512, 0, st>>>(a);
+            if (p.units > 0) paged_join_kernel<D, 256, 1><<<join, 256, 0, st>>>(a);
+        }
     } else {
-        paged_attention_kernel<D, E4M3><<<grid, 256, 0, st>>>(a);
-        if (p.units > 0) paged_join_kernel<D, 128, 1><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(a);
+        paged_attention_kernel<D, E4M3, 4><<<grid, 256, 0, st>>>(a);
+        if (p.units > 0) paged_join_kernel<D, 128, 1><<<join, 256, 0, st>>>(a);
     }
 }
 
@@ -674,7 +684,7 @@ hipError_t launch_paged_attention(const uint16_t* q, int64_t q_st, int64_t q_sh,
     PagedAttnArgs a{paged_rows(cu, B, T, table, P, kv_len, shift, num_pages, Hkv, err), q, q_st, q_sh, pool, scale, H, H / Hkv,
                     p.units, c, out, lse, nullptr, nullptr, nullptr, (int)p.grid};
     if (p.units > 0) {
-        const int64_t rows = p.grid * (p.step ? 32 : 128);
+        const int64_t rows = p.grid * p.rows;
         a.part_o = reinterpret_cast<float*>(ws);
         a.part_ml = reinterpret_cast<float2*>(ws + rows * D * 4);
         a.part_of = reinterpret_cast<int2*>(ws + rows * (D * 4 + 8));
