@@ -20,10 +20,10 @@ OBJDIR = os.path.join(LIBDIR, "obj")
 LIB = os.path.join(LIBDIR, "libmagicpig_hip.so")
 SOURCES = ["simhash.hip", "lsh.hip", "attention.hip", "prompt.hip", "paged.hip", "capi.hip"]
 ARCH = "gfx950"
-FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function"]
-# no packed f32 arithmetic (v_pk_*_f32) in these: some of its forms have returned wrong values on this part now and then
-NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCE_FLAGS = {"prompt.hip": NO_PACKED_F32, "paged.hip": NO_PACKED_F32}
+# No packed f32 arithmetic (v_pk_*_f32), which -O3 makes of ordinary f32 code by itself: some of its forms have returned wrong
+# values on this part now and then.  (The host pass says that it does not know the feature; us per layer unchanged within 0.5 %.)
+FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc() -> str:
@@ -54,7 +54,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
     def compile_one(job):
         s, o = job
-        cmd = [hipcc, *FLAGS, *SOURCE_FLAGS.get(os.path.basename(s), []), "-c", s, "-o", o]
+        cmd = [hipcc, *FLAGS, "-c", s, "-o", o]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"hipcc failed on {s}:\n{r.stdout}\n{r.stderr}")
