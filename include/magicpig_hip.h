@@ -413,8 +413,8 @@ int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_hea
  *   page_table int32 [num_seqs, pages_per_seq]  position p of request b lies in page page_table[b][p / page_size]
  *   kv_len     int32 [num_seqs]      positions of request b, the new rows included: new row i is position kv_len[b] - n_b + i
  * Rows in front of the first and behind the last request, and rows at positions below 0 (kv_len[b] < n_b), are not
- * touched; in attention the latter give 0 and -inf.  A page may belong to several requests; two rows
- * appended to one place in one call leave either.
+ * touched; in attention the latter give 0 and -inf.  A page may belong to several requests; what two rows
+ * appended to one place in one call leave there is unspecified.
  * A page id outside [0, num_pages) or a kv_len outside [0, pages_per_seq * page_size] accesses nothing outside the cache: the
  * row is skipped (append, read), or the output unspecified (attention), and mp_paged_check reports it.
  * Tensors are bf16, 16-byte aligned, read through token and head strides that are multiples of 8 elements (token strides below 2^23;

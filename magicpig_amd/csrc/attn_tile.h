@@ -274,15 +274,21 @@ struct TileOf {
 template <int BM>
 __device__ __forceinline__ TileOf find_tile(const int32_t* __restrict__ cu, int B, int T, int G, int slot) {
     auto first = [&](int i) { return (int)(((int64_t)min(max(cu[i], 0), T) * G) / BM) + i; };
-    int cnt = 0;
-    for (int base = 0; base < B; base += WAVE) {
-        const int i = base + lane_id();
-        cnt += __popcll(__ballot(i < B && first(min(i, B - 1)) <= slot));
+    // the last sequence whose first slot is not behind this one: 64 candidates at a time, the whole wave looking (one load up to
+    // 64 sequences, two up to 4096)
+    int lo = -1, n = B;                              // it is lo or one of the n behind lo
+    while (n > 0) {
+        const int step = (n + WAVE - 1) / WAVE, i = lo + 1 + lane_id() * step;
+        const int cnt = __popcll(__ballot(lane_id() * step < n && first(min(i, B - 1)) <= slot));
+        const int hit = __builtin_amdgcn_readfirstlane(cnt);
+        if (hit == 0) break;
+        n = min(step, n - (hit - 1) * step) - 1;
+        lo += 1 + (hit - 1) * step;
     }
     TileOf t;
     t.seq = -1;
     t.start = t.n = t.row0 = 0;
-    const int b = __builtin_amdgcn_readfirstlane(cnt) - 1;
+    const int b = lo;
     if (b < 0) return t;
     const int tile = slot - first(b);
     t.start = min(max(cu[b], 0), T);

@@ -1739,7 +1739,7 @@ int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_hea
                MP_ERR_INVALID, "mp_prompt_attention: strides must be multiples of 8 elements, token strides below 2^23");
     MP_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(output), MP_ERR_INVALID,
                "mp_prompt_attention: q, k, v and output must be 16-byte aligned");
-    MP_REQUIRE(num_tokens <= (1ll << 30) / (H / Hkv) && prompt_grid(num_tokens, num_seqs, H / Hkv, Hkv) < (1ll << 31) - 1,
+    MP_REQUIRE(num_tokens <= (1ll << 30) / (H / Hkv) && prompt_threads(num_tokens, num_seqs, H, Hkv, head_dim) < 1ll << 32,
                MP_ERR_UNSUPPORTED, "mp_prompt_attention: more rows than one launch can number");
     MP_HIP_CHECK(launch_prompt_attention(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v,
                                          v_token_stride, v_head_stride, cu_seqlens, num_seqs, (int)num_tokens, H, Hkv,
@@ -1819,7 +1819,7 @@ static int paged_rows_check(mp_paged_t* h, int layer_id, const int32_t* cu, int 
     MP_REQUIRE(h && h->allocated, MP_ERR_STATE, w + ": not allocated");
     MP_REQUIRE(layer_id >= 0 && layer_id < h->layers, MP_ERR_INVALID, w + ": layer_id out of range");
     MP_REQUIRE(num_seqs >= 1 && pages_per_seq >= 1 && num_tokens >= 0, MP_ERR_INVALID, w + ": bad request, page or token count");
-    MP_REQUIRE(num_tokens <= (1ll << 30) / (h->H / h->Hkv), MP_ERR_UNSUPPORTED, w + ": more rows than one launch can number");
+    MP_REQUIRE(num_tokens <= (1ll << 26) && num_tokens <= (1ll << 30) / (h->H / h->Hkv), MP_ERR_UNSUPPORTED, w + ": more rows than one launch can number");
     MP_REQUIRE(num_tokens == 0 || (cu && table && kv_len), MP_ERR_INVALID, w + ": null argument");
     return MP_OK;
 }
@@ -1878,8 +1878,8 @@ int mp_paged_attention(mp_paged_t* h, int layer_id, const uint16_t* q, int64_t q
                "mp_paged_attention: strides must be multiples of 8 elements, token strides below 2^23");
     MP_REQUIRE(aligned16(q) && aligned16(output), MP_ERR_INVALID, "mp_paged_attention: q and output must be 16-byte aligned");
     const int64_t capacity = (int64_t)pages_per_seq << h->shift;
-    MP_REQUIRE(num_tokens * h->H < (1ll << 31) - 1 &&
-                   paged_attention_grid(num_tokens, num_seqs, h->H, h->Hkv, h->D, capacity, h->cus) < (1ll << 31) - 1,
+    MP_REQUIRE(num_tokens * h->H < 1ll << 31 &&
+                   paged_attention_threads(num_tokens, num_seqs, h->H, h->Hkv, h->D, capacity, h->cus) < 1ll << 32,
                MP_ERR_UNSUPPORTED, "mp_paged_attention: more rows than one launch can number");
     const int64_t need = paged_workspace_bytes(num_tokens, num_seqs, h->H, h->Hkv, h->D, capacity, h->cus);
     MP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), MP_ERR_INVALID,

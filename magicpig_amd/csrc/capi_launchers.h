@@ -67,11 +67,11 @@ hipError_t launch_merge_state(const uint16_t*, const float*, const uint16_t*, co
                               int, uint16_t*, float*, hipStream_t);
 hipError_t launch_attn_append(const uint16_t*, const uint16_t*, const int32_t*, int, const uint16_t*, int, int, int, int64_t,
                               uint16_t*, float*, unsigned int*, int*, hipStream_t);
-int64_t prompt_grid(int64_t T, int B, int G, int Hkv);
+int64_t prompt_threads(int64_t T, int B, int H, int Hkv, int D);
 hipError_t launch_prompt_attention(const uint16_t*, int64_t, int64_t, const uint16_t*, int64_t, int64_t, const uint16_t*,
                                    int64_t, int64_t, const int32_t*, int, int, int, int, int, float, uint16_t*, float*,
                                    hipStream_t);
-int64_t paged_attention_grid(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus);
+int64_t paged_attention_threads(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus);
 int64_t paged_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus);
 hipError_t launch_paged_append(const uint16_t*, int64_t, int64_t, const uint16_t*, int64_t, int64_t, const int32_t*, int, int,
                                const int32_t*, int, const int32_t*, int, int, int, int, bool, char*, uint8_t*, int*, hipStream_t);

@@ -246,20 +246,28 @@ __device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units
     auto first = [&](int i) { return min(max(r.cu[i], 0), r.T); };
     auto row_tiles = [&](int i) { return (max(first(i + 1) - first(i), 0) * G + BM - 1) / BM; };
     auto key_tiles = [&](int i) { return (int)(((int64_t)cached(r, r.kv_len[i]) + TOK - 1) / TOK); };
-    int per = 0x3fffffff;
-    if (units > 0) {
-        float rows = 0.f, work = 0.f;           // (products of large counts; the quotient need not be exact)
-        for (int base = 0; base < r.B; base += WAVE) {
-            const int i = base + lane_id();
-            if (i >= r.B) continue;
-            const float rt = (float)row_tiles(i);
-            rows += rt;
-            work += rt * (float)key_tiles(i);
-        }
-        // half a part is lost to rounding up per tile of rows: aim so much lower that the parts still fit the chip at once
-        const float aim = fmaxf((float)units - 0.5f * wave_sum(rows), 0.5f * (float)units);
-        per = max((int)__builtin_ceilf(fminf(wave_sum(work) / aim, 1e9f)), MIN_KEYS<BM> / TOK);
+    if (units == 0) {                           // one part a tile of rows: the slots of attn_tile.h
+        const TileOf t = find_tile<BM>(r.cu, r.B, r.T, G, unit);
+        if (t.seq < 0) return p;
+        p.seq = t.seq;
+        p.start = t.start;
+        p.n = t.n;
+        p.row0 = t.row0;
+        p.kv = cached(r, r.kv_len[t.seq]);
+        p.parts = 1;
+        return p;
     }
+    float tiles = 0.f, work = 0.f;              // (products of large counts; the quotient need not be exact)
+#pragma unroll 4
+    for (int base = 0; base < r.B; base += WAVE) {
+        const int i = min(base + lane_id(), r.B - 1);
+        const float rt = base + lane_id() < r.B ? (float)row_tiles(i) : 0.f;
+        tiles += rt;
+        work += rt * (float)key_tiles(i);
+    }
+    // half a part is lost to rounding up per tile of rows: aim so much lower that the parts still fit the chip at once
+    const float aim = fmaxf((float)units - 0.5f * wave_sum(tiles), 0.5f * (float)units);
+    const int per = max((int)__builtin_ceilf(fminf(wave_sum(work) / aim, 1e9f)), MIN_KEYS<BM> / TOK);
     int before = 0;
     for (int base = 0; base < r.B; base += WAVE) {
         const int i = base + lane_id();
@@ -276,8 +284,9 @@ __device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units
             p.start = first(p.seq);
             p.n = first(p.seq + 1) - p.start;
             p.kv = cached(r, r.kv_len[p.seq]);
-            p.row0 = at / p.parts * BM;
-            p.part = at % p.parts;
+            p.row0 = at / max(p.parts, 1) * BM;
+            p.part = at % max(p.parts, 1);
+            if (p.row0 < 0 || (int64_t)p.row0 >= (int64_t)p.n * G) p.seq = -1;        // (offsets that are none)
             return p;
         }
         before = __builtin_amdgcn_readlane(sum, WAVE - 1);
@@ -646,7 +655,7 @@ PagedPlan paged_plan(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, 
     const int64_t tiles = T * G / p.rows + live, target = (p.rows == 256 ? 1 : 2) * (int64_t)cus;        // workgroups that fit the chip
     // rows alone that give every CU eight workgroups are not cut further; neither is what fits one part
     p.units = tiles * Hkv >= 4 * target || capacity <= (step ? MIN_KEYS<32> : MIN_KEYS<128>) ? 0 : (int)((target + Hkv - 1) / Hkv);
-    p.grid = (tiles + p.units + (p.units > 0)) * Hkv;
+    p.grid = (p.units > 0 ? tiles + p.units + 1 : T * G / p.rows + B) * Hkv;
     p.bytes = p.units > 0 ? p.grid * p.rows * ((int64_t)D * 4 + 8) + T * H * 8 : 0;
     return p;
 }
@@ -669,8 +678,9 @@ static void paged_attention(const PagedAttnArgs& a, const PagedPlan& p, hipStrea
     }
 }
 
-int64_t paged_attention_grid(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus) {
-    return paged_plan(T, B, H, Hkv, D, capacity, cus).grid;
+int64_t paged_attention_threads(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus) {
+    const PagedPlan p = paged_plan(T, B, H, Hkv, D, capacity, cus);
+    return p.grid * (p.rows == 256 ? 512 : 256);
 }
 int64_t paged_workspace_bytes(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, int cus) {
     return paged_plan(T, B, H, Hkv, D, capacity, cus).bytes;

@@ -154,26 +154,27 @@ __global__ __launch_bounds__(256, 2) void prompt_short_kernel(const PromptArgs a
 static bool short_prompts(int64_t T, int B, int H, int D) {
     return T * H <= 1 << 14 || (T * H <= 1 << 15 && T >= (D == 64 ? 512 : 2048) * (int64_t)B);
 }
-int64_t prompt_grid(int64_t T, int B, int G, int Hkv) { return (T * G / 32 + B) * Hkv; }       // at most
-
-template <int D, int WAVES>
-static void prompt_attention(PromptArgs a, hipStream_t st) {
-    a.slots = (int)((int64_t)a.T * a.G / (32 * WAVES) + a.B);
-    prompt_attention_kernel<D, WAVES><<<dim3((unsigned)(a.slots * a.Hkv)), 64 * WAVES, 0, st>>>(a);
+// rows of a workgroup
+static int prompt_rows(int64_t T, int B, int H, int D) {
+    if (short_prompts(T, B, H, D)) return 32;
+    return D == 128 && T * H >= WIDE_ROWS && T >= WIDE_TOKENS * B ? 256 : 128;
+}
+static int64_t prompt_slots(int64_t T, int B, int H, int Hkv, int D) { return T * (H / Hkv) / prompt_rows(T, B, H, D) + B; }
+int64_t prompt_threads(int64_t T, int B, int H, int Hkv, int D) {
+    return prompt_slots(T, B, H, Hkv, D) * Hkv * (prompt_rows(T, B, H, D) == 256 ? 512 : 256);
 }
 
 hipError_t launch_prompt_attention(const uint16_t* q, int64_t q_st, int64_t q_sh, const uint16_t* k, int64_t k_st,
                                    int64_t k_sh, const uint16_t* v, int64_t v_st, int64_t v_sh, const int32_t* cu, int B,
                                    int T, int H, int Hkv, int D, float c, uint16_t* out, float* lse, hipStream_t st) {
-    const PromptArgs a{q, k, v, q_st, q_sh, k_st, k_sh, v_st, v_sh, cu, B, T, H, Hkv, H / Hkv, 0, c, out, lse};
-    if (short_prompts(T, B, H, D)) {
-        PromptArgs b = a;
-        b.slots = (int)((int64_t)T * b.G / 32 + B);
-        if (D == 128) prompt_short_kernel<128><<<dim3((unsigned)(b.slots * Hkv)), 256, 0, st>>>(b);
-        else prompt_short_kernel<64><<<dim3((unsigned)(b.slots * Hkv)), 256, 0, st>>>(b);
-    } else if (D == 64) prompt_attention<64, 4>(a, st);
-    else if ((int64_t)T * H >= WIDE_ROWS && T >= WIDE_TOKENS * B) prompt_attention<128, 8>(a, st);
-    else prompt_attention<128, 4>(a, st);
+    const int slots = (int)prompt_slots(T, B, H, Hkv, D), rows = prompt_rows(T, B, H, D);
+    const PromptArgs a{q, k, v, q_st, q_sh, k_st, k_sh, v_st, v_sh, cu, B, T, H, Hkv, H / Hkv, slots, c, out, lse};
+    const dim3 grid((unsigned)((int64_t)slots * Hkv));
+    if (rows == 32 && D == 128) prompt_short_kernel<128><<<grid, 256, 0, st>>>(a);
+    else if (rows == 32) prompt_short_kernel<64><<<grid, 256, 0, st>>>(a);
+    else if (rows == 256) prompt_attention_kernel<128, 8><<<grid, 512, 0, st>>>(a);
+    else if (D == 128) prompt_attention_kernel<128, 4><<<grid, 256, 0, st>>>(a);
+    else prompt_attention_kernel<64, 4><<<grid, 256, 0, st>>>(a);
     return hipGetLastError();
 }
 

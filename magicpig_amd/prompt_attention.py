@@ -15,7 +15,7 @@ def rows_strides(t: torch.Tensor, heads: int, head_dim: int, name: str):
         n, h, d = t.shape
         if t.dtype is torch.bfloat16 and h == heads and d == head_dim and t.is_cuda:
             st, sh, sd = t.stride()
-            if sd == 1:
+            if sd == 1 and not (t.requires_grad and torch.is_grad_enabled()):
                 return n, st if n > 1 else heads * head_dim, sh if heads > 1 else head_dim
     except (AttributeError, ValueError):
         pass
@@ -27,7 +27,9 @@ def rows_strides(t: torch.Tensor, heads: int, head_dim: int, name: str):
         raise ValueError(f"{name}: expected shape (tokens, {heads}, {head_dim}), got {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor")
-    raise ValueError(f"{name}: the last dimension must be contiguous")
+    if t.stride(2) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    raise ValueError(f"{name}: requires a gradient, and there is no backward (torch.no_grad() for inference)")
 
 
 def same_device(index: int, **tensors) -> None:

@@ -232,6 +232,50 @@ def test_nonfinite_tokens_reach_only_rows_that_see_them(pairs, bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,B", [(8, 1, 300), (4, 2, 1100), (8, 4, 5000)])
+def test_many_requests(H, Hkv, B):
+    """One new token or none of each of B short requests: whole, and (few heads) with the keys cut."""
+    g = torch.Generator().manual_seed(35)
+    D, page, most = 64, 4, 12
+    kv = torch.randint(1, most + 1, (B,), generator=g)
+    new = (torch.arange(B) % 5 != 2).long()
+    rows = new.nonzero().flatten().cuda()
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), new.cumsum(0)]).int().cuda()
+    table = torch.randperm(B * 3, generator=g).int().view(B, 3).cuda()
+    k, v = ((torch.randn((B, most, Hkv, D), generator=g)).bfloat16().cuda() for _ in range(2))
+    q = torch.randn((int(new.sum()), H, D), generator=g).bfloat16().cuda()
+    cache = mp.PagedKVCache()
+    cache.alloc(1, H, Hkv, D, B * 3, page)
+    live = torch.arange(most)[None, :] < kv[:, None]
+    cache.append(0, k[live.cuda()], v[live.cuda()], torch.cat([torch.zeros(1, dtype=torch.long), kv.cumsum(0)]).int().cuda(), table, kv.int().cuda())
+    out, lse = cache.attention(0, q, cu, table, kv.int().cuda())
+    cache.check()
+    x = torch.einsum("bhd,bjhd->bhj", q.double(), k[rows].double().repeat_interleave(H // Hkv, 2)) / 8
+    x = x.masked_fill(~live.cuda()[rows][:, None, :], float("-inf"))
+    vv = v[rows].double().repeat_interleave(H // Hkv, 2)
+    want, mag = (torch.einsum("bhj,bjhd->bhd", x.softmax(-1), y) for y in (vv, vv.abs()))
+    attention64.check(out, want, attention64.BF16 * (want.abs() + mag) * 1.01 + 1e-4 * mag)
+    attention64.check(lse, torch.logsumexp(x, -1) / torch.log(torch.tensor(2.0, dtype=torch.float64)), torch.full_like(lse, 1e-4).double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pairs", [[(3, 900), (2, 50)], [(400, 900), (2, 50)]])
+def test_offsets_that_are_none_stay_inside(pairs):
+    """Offsets that fall, or lie outside: results are unspecified, other memory is not touched."""
+    s = Setup(pairs, 32, 16, 4, 128, "bf16", seed=36).fill()
+    T = s.T
+    for offsets in ([0, T, 1], [-9, T // 2, T + 70], [T, 0, 0], [T + 1, T + 5, T + 9]):
+        cu = torch.tensor(offsets, dtype=torch.int32).cuda()
+        whole, sums = torch.full((T + 60, 16, 128), 7.0, device="cuda", dtype=torch.bfloat16), torch.full((T + 60, 16), -3.0, device="cuda")
+        s.cache.attention(0, s.q, cu, s.table, s.kv_len, out=whole[30:T + 30], lse=sums[30:T + 30])
+        ko, vo = (torch.full((T + 60, 4, 128), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        s.cache.append(0, ko[30:T + 30], vo[30:T + 30], cu, s.table, s.kv_len)
+        s.cache.read(0, T, cu, s.table, s.kv_len, k=ko[30:T + 30], v=vo[30:T + 30])
+        for x, value in ((whole, 7.0), (sums, -3.0), (ko, 7.0), (vo, 7.0)):
+            assert bool((x[:30] == value).all()) and bool((x[T + 30:] == value).all())
+
+
+@pytest.mark.gpu
 def test_shared_pages():
     """Two requests whose first 128 positions are the same pages."""
     s = Setup([(3, 200), (5, 300)], 32, 8, 2, 128, "e4m3", seed=14)

@@ -1,5 +1,7 @@
 """prompt_attention (mp_prompt_attention) against 64 bits: lengths, head groups, strides, masked infinities, rows outside the
 sequences, streams and graphs; its refusals (CPU)."""
+import math
+
 import pytest
 import torch
 
@@ -153,6 +155,48 @@ def test_captured_on_a_side_stream_and_replayed():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [65, 700, 5000])
+def test_many_sequences(n):
+    """Every sequence is found among n, empty ones between them."""
+    lens = [(7 * i) % 4 for i in range(n)]
+    q, k, v, cu = packed(lens, 4, 2, 64, seed=33, before=1, behind=1)
+    out, lse = mp.prompt_attention(q, k, v, cu)
+    T, G = q.shape[0], 2
+    seq = torch.repeat_interleave(torch.arange(n), torch.tensor(lens)).cuda()      # all sequences as one masked product
+    x = torch.einsum("ihd,jhd->hij", q[1:-1].double(), k[1:-1].double().repeat_interleave(G, 1)) / 8
+    i = torch.arange(T - 2, device="cuda")
+    x = x.masked_fill((seq[:, None] != seq[None, :]) | (i[None, :] > i[:, None]), float("-inf"))
+    p, vv = x.softmax(-1), v[1:-1].double().repeat_interleave(G, 1)
+    want, mag = (torch.einsum("hij,jhd->ihd", p, y) for y in (vv, vv.abs()))
+    # up to 3 keys: the bound of attention64 with logits of at most 64 products of N(0, 1.5) x N(0, 2.3)
+    attention64.check(out[1:-1], want, attention64.BF16 * (want.abs() + mag) * 1.01 + 1e-4 * mag)
+    attention64.check(lse[1:-1], (torch.logsumexp(x, -1) / math.log(2.0)).t(), torch.full((T - 2, 4), 1e-4, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv", [(8, 2), (64, 8)])
+def test_offsets_that_are_none_stay_inside(H, Hkv):
+    """Offsets that fall, or lie outside: results are unspecified, memory around the outputs is not touched."""
+    q, k, v, _ = packed([600], H, Hkv, 128, seed=34)
+    for offsets in ([0, 500, 100, 600], [-70, 300, 2000], [600, 0], [900, 1000], [-5, -1], [0, 600, 600, 0, 600]):
+        whole = torch.full((800, H, 128), 7.0, device="cuda", dtype=torch.bfloat16)
+        sums = torch.full((800, H), -3.0, device="cuda")
+        mp.prompt_attention(q, k, v, torch.tensor(offsets, dtype=torch.int32).cuda(), out=whole[100:700], lse=sums[100:700])
+        for rows in (slice(0, 100), slice(700, 800)):
+            assert bool((whole[rows] == 7.0).all()) and bool((sums[rows] == -3.0).all())
+
+
+@pytest.mark.gpu
+def test_gradients_are_refused():
+    q, k, v, cu = packed([4], 8, 2, 128)
+    q.requires_grad_()
+    with pytest.raises(ValueError, match="no backward"):
+        mp.prompt_attention(q, k, v, cu)
+    with torch.no_grad():
+        mp.prompt_attention(q, k, v, cu)
+
+
+@pytest.mark.gpu
 def test_empty_inputs():
     q, k, v, cu = packed([0, 0], 8, 2, 128)
     out, lse = mp.prompt_attention(q, k, v, cu)
@@ -182,7 +226,7 @@ GOOD = dict(q=1 << 20, qt=1024, qh=128, k=1 << 20, kt=256, kh=128, v=1 << 20, vt
     (dict(q=None), 1), (dict(k=None), 1), (dict(v=None), 1), (dict(cu=None), 1), (dict(out=None), 1),
     (dict(q=(1 << 20) + 2), 1), (dict(k=(1 << 20) + 8), 1), (dict(v=(1 << 20) + 4), 1), (dict(out=(1 << 20) + 8), 1),
     (dict(qt=1020), 1), (dict(kh=12), 1), (dict(vt=-256), 1), (dict(vt=1 << 23), 1), (dict(tokens=1 << 29), 5),
-    (dict(seqs=(1 << 31) - 1), 5)])
+    (dict(seqs=(1 << 31) - 1), 5), (dict(tokens=1 << 27, H=64), 5)])
 def test_refusals_of_the_c_entry(change, code):
     a = {**GOOD, **change}
     assert L.lib().mp_prompt_attention(*(a[n] for n in GOOD)) == code
