@@ -238,60 +238,72 @@ struct PartOf {
     int part, parts;
 };
 
-template <int BM, int TOK>
-__device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units, int unit) {
+// U: requests a lane looks at, side by side (their loads are in flight together, and one scan over the wave serves 64 U of them)
+template <int BM, int TOK, int U>
+__device__ __forceinline__ PartOf find_part_of(const PagedRows& r, int G, int units, int unit) {
     PartOf p;
     p.seq = -1;
     p.start = p.n = p.row0 = p.kv = p.part = p.parts = 0;
     auto first = [&](int i) { return min(max(r.cu[i], 0), r.T); };
-    auto row_tiles = [&](int i) { return (max(first(i + 1) - first(i), 0) * G + BM - 1) / BM; };
-    auto key_tiles = [&](int i) { return (int)(((int64_t)cached(r, r.kv_len[i]) + TOK - 1) / TOK); };
-    if (units == 0) {                           // one part a tile of rows: the slots of attn_tile.h
-        const TileOf t = find_tile<BM>(r.cu, r.B, r.T, G, unit);
-        if (t.seq < 0) return p;
-        p.seq = t.seq;
-        p.start = t.start;
-        p.n = t.n;
-        p.row0 = t.row0;
-        p.kv = cached(r, r.kv_len[t.seq]);
-        p.parts = 1;
-        return p;
-    }
+    auto row_tiles = [&](int i) { return i < r.B ? (max(first(i + 1) - first(i), 0) * G + BM - 1) / BM : 0; };
+    auto key_tiles = [&](int i) { return (int)(((int64_t)cached(r, r.kv_len[min(i, r.B - 1)]) + TOK - 1) / TOK); };
     float tiles = 0.f, work = 0.f;              // (products of large counts; the quotient need not be exact)
-#pragma unroll 4
-    for (int base = 0; base < r.B; base += WAVE) {
-        const int i = min(base + lane_id(), r.B - 1);
-        const float rt = base + lane_id() < r.B ? (float)row_tiles(i) : 0.f;
-        tiles += rt;
-        work += rt * (float)key_tiles(i);
-    }
+    for (int base = 0; base < r.B; base += U * WAVE)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = base + U * lane_id() + u;
+            const float rt = (float)row_tiles(i);
+            tiles += rt;
+            work += rt * (float)key_tiles(i);
+        }
     // half a part is lost to rounding up per tile of rows: aim so much lower that the parts still fit the chip at once
     const float aim = fmaxf((float)units - 0.5f * wave_sum(tiles), 0.5f * (float)units);
-    const int per = max((int)__builtin_ceilf(fminf(wave_sum(work) / aim, 1e9f)), MIN_KEYS<BM> / TOK);
+    const float per = fmaxf(__builtin_ceilf(wave_sum(work) / aim), (float)(MIN_KEYS<BM> / TOK)), inv = 1.f / per;
     int before = 0;
-    for (int base = 0; base < r.B; base += WAVE) {
-        const int i = base + lane_id();
-        const int rt = i < r.B ? row_tiles(i) : 0, kt = rt > 0 ? key_tiles(i) : 0;
-        // (what is less than half longer than the least part is not cut)
-        const int parts = rt == 0 ? 0 : 2 * kt < 3 * (MIN_KEYS<BM> / TOK) ? 1 : (kt + per - 1) / per;
-        const int sum = before + wave_incl_scan(rt * parts);
-        const unsigned long long past = __ballot(sum > unit);
+    for (int base = 0; base < r.B; base += U * WAVE) {
+        int parts[U], units_of[U], sum = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = base + U * lane_id() + u, kt = key_tiles(i);
+            // (what is less than half longer than the least part is not cut; every workgroup rounds alike)
+            parts[u] = 2 * kt < 3 * (MIN_KEYS<BM> / TOK) ? 1 : max((int)__builtin_ceilf((float)kt * inv), 1);
+            units_of[u] = row_tiles(i) * parts[u];
+            sum += units_of[u];
+        }
+        const int upto = before + wave_incl_scan(sum);
+        const unsigned long long past = __ballot(upto > unit);
         if (past) {
             const int k = __ffsll(past) - 1;
-            p.parts = __builtin_amdgcn_readlane(parts, k);
-            const int at = unit - (__builtin_amdgcn_readlane(sum, k) - __builtin_amdgcn_readlane(rt, k) * p.parts);
-            p.seq = base + k;
+            int at = unit - (__builtin_amdgcn_readlane(upto, k) - __builtin_amdgcn_readlane(sum, k));
+            p.seq = base + U * k;
+            p.parts = __builtin_amdgcn_readlane(parts[0], k);
+#pragma unroll
+            for (int u = 0; u + 1 < U; ++u) {
+                const int here = __builtin_amdgcn_readlane(units_of[u], k);
+                if (p.seq == base + U * k + u && at >= here) {
+                    at -= here;
+                    ++p.seq;
+                    p.parts = __builtin_amdgcn_readlane(parts[u + 1], k);
+                }
+            }
             p.start = first(p.seq);
             p.n = first(p.seq + 1) - p.start;
             p.kv = cached(r, r.kv_len[p.seq]);
-            p.row0 = at / max(p.parts, 1) * BM;
-            p.part = at % max(p.parts, 1);
+            p.row0 = at / p.parts * BM;
+            p.part = at % p.parts;
             if (p.row0 < 0 || (int64_t)p.row0 >= (int64_t)p.n * G) p.seq = -1;        // (offsets that are none)
             return p;
         }
-        before = __builtin_amdgcn_readlane(sum, WAVE - 1);
+        before = __builtin_amdgcn_readlane(upto, WAVE - 1);
     }
     return p;
+}
+
+template <int BM, int TOK>
+__device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units, int unit) {
+    if (units > 0) return r.B <= WAVE ? find_part_of<BM, TOK, 1>(r, G, units, unit) : find_part_of<BM, TOK, 4>(r, G, units, unit);
+    const TileOf t = find_tile<BM>(r.cu, r.B, r.T, G, unit);        // one part a tile of rows: the slots of attn_tile.h
+    return PartOf{t.seq, t.start, t.n, t.row0, t.seq < 0 ? 0 : cached(r, r.kv_len[t.seq]), 0, 1};
 }
 
 // Many rows: 128 or 256 of one (request, kv head) a workgroup, everything else as in prompt.hip.  An e4m3 tile passes through
