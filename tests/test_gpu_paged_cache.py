@@ -180,19 +180,39 @@ def test_workgroups_of_many_rows_whole_and_in_parts(pairs, H, Hkv, D, fmt):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("pairs,H,Hkv", [([(30, 100), (1, 600)], 8, 2), ([(300, 4000), (1, 600)], 32, 8)], ids=["few rows", "many rows"])
-def test_nonfinite_values_in_every_kernel(pairs, H, Hkv):
-    s = Setup(pairs, 16, H, Hkv, 128, "bf16", seed=22)
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("pairs,H,Hkv", [([(30, 100), (1, 600)], 8, 2), ([(300, 4000), (1, 600)], 32, 8), ([(2100, 2300), (1, 600)], 32, 8)],
+                         ids=["few rows", "many rows", "most rows"])
+def test_nonfinite_values_in_every_kernel(pairs, H, Hkv, fmt):
+    s = Setup(pairs, 16, H, Hkv, 128, fmt, seed=22)
     s.v[0][-1, 0, 3] = float("inf")
     s.v[0][-2, 1, 4] = float("nan")
     s.v[0][-20, 0, 5] = float("-inf")
     s.v[1][-1, 1] = float("-inf")
     s.k[0][-3, Hkv - 1, 7] = float("nan")
     s.fill()
-    pages = s.cache.get_pages(0)[0]
-    for b, (n, kv) in enumerate(pairs):
-        pages[int(s.table[b, (kv - 1) // 16]), :, (kv - 1) % 16 + 1:] = float("nan")
+    pages, scales = s.cache.get_pages(0)
+    for b, (n, kv) in enumerate(pairs):            # what lies behind a request's end: all bits set, NaN in either format
+        place = (int(s.table[b, (kv - 1) // 16]), slice(None), slice((kv - 1) % 16 + 1, None))
+        pages.view(torch.uint8)[place] = 255
+        if scales is not None:
+            scales[place] = 255
     s.compare(*s.attend())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_pages_beyond_4_gigabytes(fmt):
+    """Requests whose pages lie at the end of a pool of more than 2^32 bytes and 2^31 elements."""
+    s = Setup([(3, 700), (200, 900)], 64, 8, 4, 128, fmt, seed=23, spare=44000 if fmt == "bf16" else 90000)
+    used = (s.table >= 0)
+    s.table[used] = (s.cache.num_pages - 1 - torch.arange(int(used.sum()), device="cuda")).int()
+    assert s.cache.footprint()["pages"] > (1 << 32) + (1 << 30)
+    s.fill()
+    s.compare(*s.attend())
+    k, v = s.cache.read(0, s.T, s.cu, s.table, s.kv_len)
+    for got, x in ((k, s.k), (v, s.v)):
+        assert torch.equal(got.double(), stored(torch.cat([x[0][-3:], x[1][-200:]]), fmt))
 
 
 @pytest.mark.gpu

@@ -155,6 +155,21 @@ def test_captured_on_a_side_stream_and_replayed():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv", [(4, 2), (32, 8)])
+def test_strides_beyond_2_to_the_31(H, Hkv):
+    """Rows 2^20 elements apart in a buffer of more than 4 GB."""
+    q, k, v, cu = packed([2000, 150], H, Hkv, 64, seed=37)
+    buf = torch.empty(2150 << 20, dtype=torch.bfloat16, device="cuda")
+    wide, at = [], 0
+    for x in (q, k, v):
+        wide.append(buf.as_strided(x.shape, (1 << 20, 64, 1), at))
+        wide[-1].copy_(x)
+        at += x.shape[1] * 64
+    want, got = mp.prompt_attention(q, k, v, cu), mp.prompt_attention(*wide, cu)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [65, 700, 5000])
 def test_many_sequences(n):
     """Every sequence is found among n, empty ones between them."""
