@@ -252,15 +252,22 @@ __device__ __forceinline__ void add_values(RowState<D>& st, const bf16x8 (&p)[2 
     }
     if (MASK && odd) add_nonfinite<D, SUB>(st.o, vt, lim);
 }
-template <int D, int SUB, bool MASK>
-__device__ __forceinline__ void fold_tile(RowState<D>& st, const char* kt, const char* vt, float c, int lim) {
+// All of them.  `between` runs behind the first product.
+template <int D, int SUB, bool MASK, class F>
+__device__ __forceinline__ void fold_tile(RowState<D>& st, const char* kt, const char* vt, float c, int lim, F between) {
     f32x16 s[SUB];
     bf16x8 p[2 * SUB];
     tile_scores<D, SUB>(s, st, kt);
+    between();
     if (MASK) mask_scores<SUB>(s, lim);
     const float sum = tile_weights<D, SUB>(st, s, c, p);
     settle_weights<D, SUB>(st, s, c, p, sum);
     add_values<D, SUB, MASK>(st, p, vt, lim);
+}
+
+template <int D, int SUB, bool MASK>
+__device__ __forceinline__ void fold_tile(RowState<D>& st, const char* kt, const char* vt, float c, int lim) {
+    fold_tile<D, SUB, MASK>(st, kt, vt, c, lim, [] {});
 }
 
 // Which sequence and which of its tiles a slot is.  Sequence b of rows cu[b] G .. cu[b + 1] G owns the slots from
