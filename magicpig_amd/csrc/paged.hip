@@ -227,9 +227,9 @@ struct PagedAttnArgs {
 template <int BM>
 constexpr int MIN_KEYS = BM == 32 ? 256 : 512;
 
-// From here on 256 rows a workgroup at head_dim 128, which read the keys from L2 half as often: 4096 new tokens of 32 heads over 8
-// behind 32 000 1.99 ms against 2.12, 16 x 512 of 8 heads over 1 behind 2000 (e4m3) 82 us against 88; at the border itself it is
-// even (2048 of 32 heads behind 32 000 1.05 ms against 1.11, behind 67 584 2.33 against 2.30).
+// From here on 256 rows a workgroup at head_dim 128, which read the keys from L2 half as often: 2048 new tokens of 32 heads over 8
+// behind 67 584 2.12 ms against 2.30, 16 x 512 of 8 heads over 1 behind 2000 (e4m3) 81 us against 86.  (Where all keys are new and few
+// heads share a chip, the shorter workgroups pack better: 8192 of 8 heads over 1, e4m3, 241 us against 232.)
 constexpr int64_t WIDE_ROWS = 1 << 16;
 
 struct PartOf {
@@ -286,12 +286,13 @@ __device__ __forceinline__ PartOf find_part_of(const PagedRows& r, int G, int un
                     p.parts = __builtin_amdgcn_readlane(parts[u + 1], k);
                 }
             }
+            p.seq = min(p.seq, r.B - 1);                                     // (offsets that are none could count past the end)
             p.start = first(p.seq);
             p.n = first(p.seq + 1) - p.start;
             p.kv = cached(r, r.kv_len[p.seq]);
             p.row0 = at / p.parts * BM;
             p.part = at % p.parts;
-            if (p.row0 < 0 || (int64_t)p.row0 >= (int64_t)p.n * G) p.seq = -1;        // (offsets that are none)
+            if (p.row0 < 0 || (int64_t)p.row0 >= (int64_t)p.n * G) p.seq = -1;
             return p;
         }
         before = __builtin_amdgcn_readlane(upto, WAVE - 1);
@@ -302,7 +303,8 @@ __device__ __forceinline__ PartOf find_part_of(const PagedRows& r, int G, int un
 template <int BM, int TOK>
 __device__ __forceinline__ PartOf find_part(const PagedRows& r, int G, int units, int unit) {
     if (units > 0) return r.B <= WAVE ? find_part_of<BM, TOK, 1>(r, G, units, unit) : find_part_of<BM, TOK, 4>(r, G, units, unit);
-    const TileOf t = find_tile<BM>(r.cu, r.B, r.T, G, unit);        // one part a tile of rows: the slots of attn_tile.h
+    // one part a tile of rows: the slots of attn_tile.h, a request's longest first
+    const TileOf t = find_tile<BM>(r.cu, r.B, r.T, G, (int)(gridDim.x / r.Hkv) - 1 - unit);
     return PartOf{t.seq, t.start, t.n, t.row0, t.seq < 0 ? 0 : cached(r, r.kv_len[t.seq]), 0, 1};
 }
 
@@ -670,7 +672,7 @@ PagedPlan paged_plan(int64_t T, int B, int H, int Hkv, int D, int64_t capacity, 
     // them again, which costs less than the few, long workgroups of 128 rows as long as it is little in all: 16 new tokens of one
     // request, 32 heads over 8, behind 2000 tokens: 12.8 us against 19.8; behind 8000 (2^17 tokens x tiles) 21.4 against
     // 24.4; behind 32 000 50 against 42; 8 such requests behind 2000 (2^18) 31 against 26.  (The host knows the tables' size, not the lengths.)
-    const bool step = T * G <= 32 * live || (T * G + 31) / 32 * Hkv * capacity <= 1 << 17;
+    const bool step = T * G <= 32 * live || (T * G + 31) / 32 * Hkv <= (1 << 17) / capacity;
     p.rows = step ? 32 : D == 128 && T * H >= WIDE_ROWS ? 256 : 128;
     const int64_t tiles = T * G / p.rows + live, target = (p.rows == 256 ? 1 : 2) * (int64_t)cus;        // workgroups that fit the chip
     // rows alone that give every CU eight workgroups are not cut further; neither is what fits one part
