@@ -28,9 +28,10 @@ template <int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const PromptArgs a) {
     constexpr int THREADS = 64 * WAVES, BM = 32 * WAVES, CPR = D / 8, PASSES = TILE_TOKENS * CPR / THREADS, KB = TILE_TOKENS * 2 * D;
     __shared__ __attribute__((aligned(1024))) char lds[2][2][KB];      // [buffer][K, V]
-    // heads fastest: with 8 kv heads the workgroups of one head meet in one XCD's L2; longest rows of a sequence first
-    const int head = blockIdx.x % a.Hkv;
-    const TileOf t = find_tile<BM>(a.cu, a.B, a.T, a.G, a.slots - 1 - (int)(blockIdx.x / a.Hkv));
+    // heads fastest: with 8 kv heads the workgroups of one head meet in one XCD's L2; the longest first
+    const int head = blockIdx.x % a.Hkv, at = (int)(blockIdx.x / a.Hkv);
+    const TileOf t = a.B > 1 && a.B <= WAVE ? find_tile_longest_first<BM>(a.cu, a.B, a.T, a.G, at)
+                                            : find_tile<BM>(a.cu, a.B, a.T, a.G, a.slots - 1 - at);
     if (t.seq < 0) return;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane_id();
     const int rows = t.n * a.G;

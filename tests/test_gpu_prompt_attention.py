@@ -189,6 +189,19 @@ def test_many_sequences(n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B", [2, 63, 64, 65])
+@pytest.mark.parametrize("H,Hkv", [(32, 8), (7, 1)])
+def test_uneven_sequences_on_both_sides_of_a_wave(B, H, Hkv):
+    """Lengths of 0 to 700 in mixed order; a lane stands for a sequence while they are at most 64."""
+    lens = [(i * 389 + 650) % 701 if i % 5 != 3 else i % 2 for i in range(B)]
+    q, k, v, cu = packed(lens, H, Hkv, 64, seed=B, before=1, behind=2)
+    out, lse = torch.full_like(q, 7.0), torch.full((q.shape[0], H), -3.0, device="cuda")
+    mp.prompt_attention(q, k, v, cu, out=out, lse=lse)
+    compare(q, k, v, cu, out, lse)
+    assert bool((out[0] == 7.0).all()) and bool((out[-2:] == 7.0).all()) and bool((lse[-2:] == -3.0).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,Hkv", [(8, 2), (64, 8)])
 def test_offsets_that_are_none_stay_inside(H, Hkv):
     """Offsets that fall, or lie outside: results are unspecified, memory around the outputs is not touched."""
