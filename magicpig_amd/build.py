@@ -3,7 +3,7 @@
     python -m magicpig_amd.build [--force]
 
 hipcc cross-compiles without a GPU.  The library is written IN-TREE
-(magicpig_amd/lib/libmagicpig_hip.so) so it travels to the GPU box with the source snapshot.
+(magicpig_amd/lib/libmagicpig_hip.so) so a copy of the tree carries it.
 """
 from __future__ import annotations
 
