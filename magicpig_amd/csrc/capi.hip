@@ -1812,15 +1812,20 @@ int mp_paged_alloc(mp_paged_t* h, int num_layers, int num_attention_heads, int n
     return MP_OK;
 }
 
-// what append, read and attention check alike
+// rows that the kernels number in 32 bits (2^30 rows of a kv head; a copy's workgroups)
+static bool paged_tokens_ok(const mp_paged_t* h, int64_t num_tokens) {
+    return num_tokens <= 1ll << 26 && num_tokens <= (1ll << 30) / (h->H / h->Hkv);
+}
+// what append, read and attention check alike (a message is made only where a check fails)
 static int paged_rows_check(mp_paged_t* h, int layer_id, const int32_t* cu, int num_seqs, int64_t num_tokens,
                             const int32_t* table, int pages_per_seq, const int32_t* kv_len, const char* who) {
-    const std::string w(who);
-    MP_REQUIRE(h && h->allocated, MP_ERR_STATE, w + ": not allocated");
-    MP_REQUIRE(layer_id >= 0 && layer_id < h->layers, MP_ERR_INVALID, w + ": layer_id out of range");
-    MP_REQUIRE(num_seqs >= 1 && pages_per_seq >= 1 && num_tokens >= 0, MP_ERR_INVALID, w + ": bad request, page or token count");
-    MP_REQUIRE(num_tokens <= (1ll << 26) && num_tokens <= (1ll << 30) / (h->H / h->Hkv), MP_ERR_UNSUPPORTED, w + ": more rows than one launch can number");
-    MP_REQUIRE(num_tokens == 0 || (cu && table && kv_len), MP_ERR_INVALID, w + ": null argument");
+#define MP_PAGED_REQUIRE(cond, code, msg) MP_REQUIRE(cond, code, std::string(who) + (msg))
+    MP_PAGED_REQUIRE(h && h->allocated, MP_ERR_STATE, ": not allocated");
+    MP_PAGED_REQUIRE(layer_id >= 0 && layer_id < h->layers, MP_ERR_INVALID, ": layer_id out of range");
+    MP_PAGED_REQUIRE(num_seqs >= 1 && pages_per_seq >= 1 && num_tokens >= 0, MP_ERR_INVALID, ": bad request, page or token count");
+    MP_PAGED_REQUIRE(paged_tokens_ok(h, num_tokens), MP_ERR_UNSUPPORTED, ": more rows than one launch can number");
+    MP_PAGED_REQUIRE(num_tokens == 0 || (cu && table && kv_len), MP_ERR_INVALID, ": null argument");
+#undef MP_PAGED_REQUIRE
     return MP_OK;
 }
 
@@ -1860,6 +1865,7 @@ int mp_paged_read(mp_paged_t* h, int layer_id, uint16_t* k, uint16_t* v, const i
 int mp_paged_workspace(mp_paged_t* h, int num_seqs, int64_t num_tokens, int pages_per_seq, int64_t* bytes) {
     MP_REQUIRE(h && h->allocated, MP_ERR_STATE, "mp_paged_workspace: not allocated");
     MP_REQUIRE(bytes && num_seqs >= 1 && pages_per_seq >= 1 && num_tokens >= 0, MP_ERR_INVALID, "mp_paged_workspace: bad argument");
+    MP_REQUIRE(paged_tokens_ok(h, num_tokens), MP_ERR_UNSUPPORTED, "mp_paged_workspace: more rows than one launch can number");
     *bytes = paged_workspace_bytes(num_tokens, num_seqs, h->H, h->Hkv, h->D, (int64_t)pages_per_seq << h->shift, h->cus);
     return MP_OK;
 }

@@ -456,6 +456,9 @@ def test_refusals_of_calls():
     need = C.c_int64()
     L.check(L.lib().mp_paged_workspace(long.cache._h, 1, 1, long.table.shape[1], C.byref(need)))
     assert need.value > 0
+    for tokens in ((1 << 26) + 1, (1 << 63) - 1):
+        assert L.lib().mp_paged_workspace(long.cache._h, 1, tokens, 1, C.byref(C.c_int64())) == 5      # as the call itself
+        assert L.lib().mp_paged_append(long.cache._h, 0, 16, 256, 128, 16, 256, 128, 16, 1, tokens, 16, 1, 16, None) == 5
     o = torch.empty_like(long.q)
     for ptr, size in ((None, 0), (o.data_ptr(), need.value - 1), (o.data_ptr() + 8, need.value)):
         assert L.lib().mp_paged_attention(long.cache._h, 0, L.ptr(long.q), 1024, 128, L.ptr(long.cu), 1, 1, L.ptr(long.table),
