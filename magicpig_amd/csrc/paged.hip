@@ -23,14 +23,16 @@ struct PagedRows {
     int* err;
 };
 
-// a request's cache length, inside what its table can hold
+// whether a request's table can hold this length
+__device__ __forceinline__ int table_positions(const PagedRows& r) { return (int)min((int64_t)r.P << r.shift, (int64_t)0x7fffffff); }
+__device__ __forceinline__ bool length_ok(const PagedRows& r, int want) {
+    if (want >= 0 && want <= table_positions(r)) return true;
+    atomicOr(r.err, 1);
+    return false;
+}
+// a request's cache length for attention, which only reads: the nearest that its table can hold
 __device__ __forceinline__ int cached(const PagedRows& r, int want) {
-    const int have = (int)min((int64_t)r.P << r.shift, (int64_t)0x7fffffff);
-    if (want < 0 || want > have) {
-        atomicOr(r.err, 1);
-        return want < 0 ? 0 : have;
-    }
-    return want;
+    return length_ok(r, want) ? want : want < 0 ? 0 : table_positions(r);
 }
 // page id -> a page that exists
 __device__ __forceinline__ int page_ok(const PagedRows& r, int page) {
@@ -110,7 +112,9 @@ __global__ __launch_bounds__(256) void paged_copy_kernel(const CopyArgs a) {
         }
         uint32_t at = NO_ROW;
         if (lo < r.B && cu(lo) <= tok) {
-            const int pos = cached(r, small ? s_kv[lo] : r.kv_len[lo]) - min(cu(lo + 1), r.T) + tok;
+            // (the rows of a length that the table cannot hold have no place: any other would be another position's)
+            const int len = small ? s_kv[lo] : r.kv_len[lo];
+            const int pos = length_ok(r, len) ? len - min(cu(lo + 1), r.T) + tok : -1;
             if (pos >= 0) {
                 const int page = page_ok(r, r.table[(int64_t)lo * r.P + (pos >> r.shift)]);
                 if (page >= 0) at = (((uint32_t)page * (uint32_t)r.Hkv) << r.shift) | (uint32_t)(pos & ((1 << r.shift) - 1));

@@ -386,6 +386,38 @@ def test_bad_pages_and_lengths_are_reported():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("more", [0, 300], ids=["few requests", "many requests"])
+def test_rows_past_the_table_are_skipped(more, D, fmt):
+    """A request that fills its table, and lengths that the table cannot hold: no byte of the pages changes, read leaves its
+    outputs, and the next calls are as before.  Its last page is also the first of another request."""
+    s = Setup([(0, 112), (2, 90)] + [(0, 1)] * more, 16, 4, 2, D, fmt, seed=18)
+    s.table[1, 0] = s.table[0, 6]
+    s.k[1][:16], s.v[1][:16] = s.k[0][96:], s.v[0][96:]
+    s.fill()
+    whole = [x.view(torch.uint8).clone() for x in s.cache.get_pages(0) if x is not None]
+    for new, length in ((1, 113), (5, 115), (3, 113), (16, 112 + 16), (1, (1 << 31) - 1), (2, -1), (1, -(1 << 31))):
+        kv_len = s.kv_len.clone()
+        kv_len[0] = length
+        cu = torch.tensor([0] + [new] + [new + 2] * (more + 1), dtype=torch.int32).cuda()
+        junk = torch.full((new, 2, D), 3.0, dtype=torch.bfloat16, device="cuda")
+        s.cache.append(0, torch.cat([junk, s.k[1][-2:]]), torch.cat([junk, s.v[1][-2:]]), cu, s.table, kv_len)    # (request 1 as it is)
+        for now, then in zip((x for x in s.cache.get_pages(0) if x is not None), whole):
+            assert torch.equal(now.view(torch.uint8), then), f"{new} rows, kv_len {length}"
+        with pytest.raises(mp.MagicPigError, match="MP_ERR_DATA.*kv_len"):
+            s.cache.check()
+        ko, vo = (torch.full((new + 2, 2, D), 9.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        s.cache.read(0, new + 2, cu, s.table, kv_len, k=ko, v=vo)
+        for got, x in ((ko, s.k[1]), (vo, s.v[1])):
+            assert bool((got[:new] == 9.0).all()), f"{new} rows, kv_len {length}"
+            assert torch.equal(got[new:].double(), stored(x[-2:], fmt))
+        with pytest.raises(mp.MagicPigError, match="MP_ERR_DATA.*kv_len"):
+            s.cache.check()
+    s.compare(*s.attend())
+
+
+@pytest.mark.gpu
 def test_no_new_rows():
     s = Setup([(0, 100), (0, 3)], 16, 8, 2, 128, "bf16").fill()
     out, lse = s.attend()
