@@ -394,8 +394,8 @@ int mp_decode_layer_window_ex(mp_simhash_t* s, mp_lsh_t* lsh, mp_attn_t* attn, m
  *   empty; rows in front of the first and behind the last sequence are not read and their outputs stay as they were;
  *   output bf16 [num_tokens, H, D], lse f32 [num_tokens, H] (base-2 log-sum-exp, may be NULL), contiguous.
  * Token i of a sequence sees its tokens 0 .. i; query head h reads kv head h / (H / Hkv).  head_dim 64 or 128; scale > 0.
- * An infinity or NaN in a key or value reaches the rows that see it and no others.  Offsets that decrease or leave
- * [0, num_tokens] are clamped (no access outside the tensors), the results are then unspecified.  Device pointers only, work
+ * An infinity or NaN in a key or value reaches the rows that see it and no others; a row all of whose logits are -inf gives NaN
+ * and a log-sum-exp of -inf, as 0 / 0 does.  Offsets that decrease or leave [0, num_tokens] are clamped (no access outside the tensors), the results are then unspecified.  Device pointers only, work
  * is enqueued on `stream` of the current device; no state, no workspace: calls may overlap and be captured. */
 int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
                         int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v, int64_t v_token_stride,

@@ -338,17 +338,21 @@ __device__ __forceinline__ TileOf find_tile_longest_first(const int32_t* __restr
     return t;
 }
 
+// 1 / l for a row's output.  A row that sees nothing is 0.  One that sees keys but whose weights are all 0 sees logits of -inf
+// alone, and 0 / 0 is NaN: what the definition gives (its log-sum-exp is -inf as well).
+__device__ __forceinline__ float inverse_sum(float l, bool sees) { return sees ? 1.f / l : 0.f; }
+
 // Base-2 log-sum-exp of sum l over 2^m: -inf of nothing, +inf where a logit was (its weights are NaN, as inf - inf is).
 __device__ __forceinline__ float log_sum(float m, float l) {
     return l == 0.f ? NEG_INF : m == __builtin_inff() ? m : m + __builtin_amdgcn_logf(l);
 }
 
-// The wave's rows as they leave: normalised, bf16, with the base-2 log-sum-exp; a row that saw nothing is 0 and -inf.
+// The wave's rows as they leave: normalised, bf16, with the base-2 log-sum-exp; `sees`: there is a key that the row may see.
 template <int D>
-__device__ __forceinline__ void store_rows(const RowState<D>& st, uint16_t* out, float* lse) {     // this lane's row
+__device__ __forceinline__ void store_rows(const RowState<D>& st, uint16_t* out, float* lse, bool sees) {     // this lane's row
     const int h = lane_id() >> 5;
     const float l = halves_sum(st.l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = inverse_sum(l, sees);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
@@ -406,8 +410,8 @@ __device__ __forceinline__ void join_waves(const RowState<D>& st, f32x4* mine, c
 }
 // ... and as they leave: this thread's chunks of its row
 template <int D>
-__device__ __forceinline__ void store_chunks(uint16_t* out, const f32x4 (&o)[D / 32], float total) {
-    const float inv = total == 0.f ? 0.f : 1.f / total;
+__device__ __forceinline__ void store_chunks(uint16_t* out, const f32x4 (&o)[D / 32], float total, bool sees) {
+    const float inv = inverse_sum(total, sees);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
         u32x2 b;

@@ -412,9 +412,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_attention_kernel(const Pa
 
     if (wrow + (l & 31) >= rows) return;
     const int64_t orow = (int64_t)(t.start + tok) * a.H + h;
-    if (a.units > 0 && t.part == 0 && l < 32) a.part_of[orow] = make_int2((int)blockIdx.x * BM + 32 * w + l, used);
-    if (used == 1) {
-        store_rows<D>(st, a.out + orow * D, a.lse ? a.lse + orow : nullptr);
+    // (a row that sees nothing, though others of its tile see more than one part, leaves with the first: nothing to join)
+    const bool whole_row = used == 1 || (lim < 0 && t.part == 0);
+    if (a.units > 0 && t.part == 0 && l < 32) a.part_of[orow] = make_int2((int)blockIdx.x * BM + 32 * w + l, whole_row ? 1 : used);
+    if (whole_row) {
+        store_rows<D>(st, a.out + orow * D, a.lse ? a.lse + orow : nullptr, lim >= 0);
         return;
     }
     const int64_t prow = (int64_t)blockIdx.x * BM + 32 * w + (l & 31);
@@ -524,12 +526,12 @@ __global__ __launch_bounds__(256, 2) void paged_step_kernel(const PagedAttnArgs 
     if (grow >= rows) return;
     const int64_t orow = (int64_t)(t.start + grow / a.G) * a.H + head * a.G + grow % a.G;
     const int64_t prow = (int64_t)blockIdx.x * BM + r;
-    if (used > 1) {
+    if (used > 1) {                      // (32 rows and more than a tile of keys: each row sees some)
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
             *reinterpret_cast<f32x4*>(a.part_o + prow * D + 4 * ((threadIdx.x & 7) * (D / 32) + c)) = o[c];
     } else {
-        store_chunks<D>(a.out + orow * D, o, total);
+        store_chunks<D>(a.out + orow * D, o, total, old + grow / a.G >= 0);
     }
     if ((threadIdx.x & 7) != 0) return;
     if (a.units > 0 && t.part == 0) a.part_of[orow] = make_int2((int)blockIdx.x * BM + r, used);
@@ -611,7 +613,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
         }
     }
     if (n == 0) return;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = inverse_sum(sum, true);
     if (W == 2) *reinterpret_cast<uint32_t*>(a.out + row * D + 2 * l) = pack_bf16(o[0] * inv, o[W - 1] * inv);
     else a.out[row * D + l] = (uint16_t)(pack_bf16(o[0] * inv, 0.f) & 0xffffu);
     if (a.lse != nullptr && l == 0) a.lse[row] = log_sum(m, sum);

@@ -75,7 +75,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(const P
     }
     if (wrow + (l & 31) >= rows) return;
     const int64_t orow = (int64_t)(t.start + tok) * a.H + h;
-    store_rows<D>(st, a.out + orow * D, a.lse ? a.lse + orow : nullptr);
+    store_rows<D>(st, a.out + orow * D, a.lse ? a.lse + orow : nullptr, true);      // (itself at least)
 }
 
 // Short prompts: too few workgroups of 128 rows to fill the chip, each walking its keys alone.  Here a workgroup owns 32 rows
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(256, 2) void prompt_short_kernel(const PromptArgs a
     join_waves<D>(st, reinterpret_cast<f32x4*>(lds[w]), reinterpret_cast<const f32x4*>(lds[0]), 2 * KB / 16, ml, m, total, o);
     if (grow >= rows) return;
     const int64_t orow = (int64_t)(t.start + grow / a.G) * a.H + head * a.G + grow % a.G;
-    store_chunks<D>(a.out + orow * D, o, total);
+    store_chunks<D>(a.out + orow * D, o, total, true);
     if (a.lse != nullptr && (threadIdx.x & 7) == 0) a.lse[orow] = log_sum(m, total);
 }
 

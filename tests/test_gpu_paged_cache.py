@@ -201,6 +201,24 @@ def test_nonfinite_values_in_every_kernel(pairs, H, Hkv, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("pairs,H,Hkv", [
+    ([(1, 9000), (3, 70)], 8, 2), ([(33, 600), (2, 0), (5, 3)], 8, 2), ([(300, 4000), (800, 750)], 8, 8), ([(400, 460), (400, 90)], 32, 8),
+    ([(2100, 2300), (500, 40)], 32, 8)], ids=["step in parts", "step", "parts, a row that sees nothing", "128", "256"])
+def test_rows_whose_logits_are_all_minus_infinity(pairs, H, Hkv, D):
+    """Every key of a request, or its first 64, hold an infinity that makes all logits of some rows -inf: 0 / 0 there, log-sum-exp
+    -inf; 0 and -inf where a row sees no key at all."""
+    s = Setup(pairs, 16, H, Hkv, D, "bf16", seed=24)
+    s.k[0][:, 0, 3] = float("inf")
+    s.k[-1][:64, 0, 3] = float("inf")
+    s.q[:, :H // Hkv, 3] = -s.q[:, :H // Hkv, 3].abs() - 0.5
+    s.fill()
+    out, lse = s.attend()
+    assert bool(torch.isnan(out[0, 0]).all()) and float(lse[0, 0]) == float("-inf")
+    s.compare(out, lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 def test_pages_beyond_4_gigabytes(fmt):
     """Requests whose pages lie at the end of a pool of more than 2^32 bytes and 2^31 elements."""

@@ -119,6 +119,21 @@ def test_nonfinite_tokens_reach_only_rows_that_see_them(bad, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,Hkv", SIZES, ids=["32", "128", "256"])
+def test_rows_whose_logits_are_all_minus_infinity(lens, H, Hkv, D):
+    """The first keys of a sequence hold an infinity: a row that sees nothing but logits of -inf is 0 / 0, its log-sum-exp -inf;
+    rows behind them have a weight of 0 there."""
+    q, k, v, cu = packed(lens, H, Hkv, D, seed=38)
+    for a, n in ((cu[0], 40), (cu[2] if len(lens) > 2 else cu[1], 100)):
+        k[a:a + n, 0, 3] = float("inf")
+        q[a:, :H // Hkv, 3] = -q[a:, :H // Hkv, 3].abs() - 0.5
+    out, lse = mp.prompt_attention(q, k, v, cu)
+    assert bool(torch.isnan(out[0, 0]).all()) and float(lse[0, 0]) == float("-inf")
+    compare(q, k, v, cu, out, lse)
+
+
+@pytest.mark.gpu
 def test_peaked_and_flat_rows():
     """Logits of thousands next to zeros: the maximum moves far and late, weights underflow."""
     q, k, v, cu = packed([500], 4, 2, 128, seed=8)
