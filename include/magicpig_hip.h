@@ -394,8 +394,11 @@ int mp_decode_layer_window_ex(mp_simhash_t* s, mp_lsh_t* lsh, mp_attn_t* attn, m
  *   empty; rows in front of the first and behind the last sequence are not read and their outputs stay as they were;
  *   output bf16 [num_tokens, H, D], lse f32 [num_tokens, H] (base-2 log-sum-exp, may be NULL), contiguous.
  * Token i of a sequence sees its tokens 0 .. i; query head h reads kv head h / (H / Hkv).  head_dim 64 or 128; scale > 0.
- * An infinity or NaN in a key or value reaches the rows that see it and no others; a row all of whose logits are -inf gives NaN
- * and a log-sum-exp of -inf, as 0 / 0 does.  Offsets that decrease or leave [0, num_tokens] are clamped (no access outside the tensors), the results are then unspecified.  Device pointers only, work
+ * Logits, weights' sums and outputs are summed in f32; the weights are rounded to bf16 for the product with V, so an output is off
+ * by up to 2^-8 of sum |weight v| and 2^-8 of itself (its own rounding).  Finite inputs give finite results while every
+ * |scale q . k| is below 2^24 and every |v| below 2^120 / (tokens the row sees).  An infinity or NaN in a key or value reaches the
+ * rows that see it and no others: an infinity in V comes out as an infinity, or as NaN where its weight is too small for f32
+ * (0 * inf); a row all of whose logits are -inf gives NaN and a log-sum-exp of -inf, as 0 / 0 does.  Offsets that decrease or leave [0, num_tokens] are clamped (no access outside the tensors), the results are then unspecified.  Device pointers only, work
  * is enqueued on `stream` of the current device; no state, no workspace: calls may overlap and be captured. */
 int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
                         int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v, int64_t v_token_stride,
@@ -427,7 +430,8 @@ int mp_paged_alloc(mp_paged_t* h, int num_layers, int num_attention_heads, int n
                    int64_t num_pages, int page_size, int kv_format);
 /* k, v [num_tokens, Hkv, D] into the pages.  MP_KV_E4M3: a row (one head's K or V of a token) is stored as e4m3(x 2^-e) and e,
  * the least integer >= -126 with max |x| <= 448 * 2^e; codes round to nearest even, products with 2^e are exact (where the
- * result is a normal bf16 number).  Infinities and NaN become NaN and do not count for the maximum. */
+ * result is a normal bf16 number; magnitudes of 2^128 (1 - 2^-5) and more round up to 2^128, which bf16 holds as an infinity).
+ * Infinities and NaN become NaN and do not count for the maximum. */
 int mp_paged_append(mp_paged_t* h, int layer_id, const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
                     const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens, int num_seqs,
                     int64_t num_tokens, const int32_t* page_table, int pages_per_seq, const int32_t* kv_len,
@@ -440,7 +444,8 @@ int mp_paged_read(mp_paged_t* h, int layer_id, uint16_t* k, uint16_t* v, const i
  * q [num_tokens, H, D]; output bf16 [num_tokens, H, D]; lse f32 [num_tokens, H] (base 2, may be NULL); scale > 0.
  * workspace: at least mp_paged_workspace(...) bytes, 16-byte aligned, not shared with a call that may run at the same time
  * (may be NULL where that is 0); its contents need no preparation.  The keys of a row are split over workgroups when the
- * rows are few, and joined in a fixed order: results do not vary from run to run. */
+ * rows are few, and joined in a fixed order: results do not vary from run to run.  Precision, range and what infinities and NaN
+ * give are mp_prompt_attention's; a row that sees no position gives 0 and -inf. */
 int mp_paged_workspace(mp_paged_t* h, int num_seqs, int64_t num_tokens, int pages_per_seq, int64_t* bytes);
 int mp_paged_attention(mp_paged_t* h, int layer_id, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                        const int32_t* cu_seqlens, int num_seqs, int64_t num_tokens, const int32_t* page_table,

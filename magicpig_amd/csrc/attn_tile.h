@@ -9,8 +9,10 @@
 //     m' = max(m, max_j x_j),  l' = 2^(m - m') l + sum_j 2^(x_j - m'),  o' = 2^(m - m') o + sum_j 2^(x_j - m') v_j
 // and end with o / l and the base-2 log-sum-exp m + log2 l.  m need not be the maximum, only near or above it: the weights
 // are made with the m there is, and only where a lane's share of a tile's weights sums to more than 1024 (or the row has seen
-// nothing yet) is the maximum looked for, m moved, o and l scaled and the weights made again.  Larger weights change neither f32
-// sums nor the relative precision of a bf16 weight, and most tiles cost no maximum and no scaling (3 % at 32 768 tokens).
+// nothing yet) is the maximum looked for, m moved, o and l scaled and the weights made again.  Larger weights change neither the
+// relative precision of f32 sums nor that of a bf16 weight, and most tiles cost no maximum and no scaling (3 % at 32 768 tokens).
+// They cost range: over n keys l stays below 128 n (2048 a tile of 32 keys or more; 2 n of one tile), so o is finite for
+// |v| < 2^120 / n.  m is rounded to f32, which moves a weight by 2^+-1 at most while |x| < 2^25.
 // m, l, o are f32; the weights 2^(x - m) are rounded to bf16 once, for the second matrix product (relative error 2^-8 each at
 // most, as the output's own rounding); l sums them unrounded.
 //

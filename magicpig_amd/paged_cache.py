@@ -37,7 +37,8 @@ class PagedKVCache:
               page_size: int = 64, kv_format: str = "bf16") -> None:
         """Pages of `page_size` tokens (a power of two up to 4096) for `num_layers` layers on the current device.
         kv_format "e4m3": a row -- one head's K or V of a token -- becomes e4m3 codes and one power of two, half the memory;
-        an element then comes back off by at most 2^-4 of itself, or 2^-17 of its row's largest where that is more."""
+        an element then comes back off by at most 2^-4 of itself, or 2^-17 of its row's largest where that is more (magnitudes
+        of 2^128 (1 - 2^-5) and more, the top of bf16's range, come back as infinities)."""
         if kv_format not in L.KV_FORMATS:
             raise ValueError(f"kv_format: expected one of {sorted(L.KV_FORMATS)}, got {kv_format!r}")
         L.check(L.lib().mp_paged_alloc(self._h, num_layers, num_attention_heads, num_key_value_heads, head_dim, num_pages,
@@ -89,7 +90,8 @@ class PagedKVCache:
                   lse: torch.Tensor | None = None):
         """q bf16 [T, H, D]: row cu_seqlens[b] + i attends to positions 0 .. kv_len[b] - n_b + i of request b, as the pages hold
         them (append the rows' own keys first); query head h to kv head h // (H // Hkv).  Returns (out bf16 [T, H, D],
-        lse f32 [T, H], base 2); a row that sees nothing gives 0 and -inf.  scale: default head_dim ** -0.5."""
+        lse f32 [T, H], base 2); a row that sees nothing gives 0 and -inf.  scale: default head_dim ** -0.5.  Sums are f32, the
+        weights are rounded to bf16 for the product with v."""
         H, D = self.H, self.D
         T, qt, qh = rows_strides(q, H, D, "q")
         if out is None:

@@ -219,6 +219,27 @@ def test_rows_whose_logits_are_all_minus_infinity(pairs, H, Hkv, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pairs,H,Hkv", [([(1, 9000), (5, 700)], 8, 2), ([(300, 4000), (1, 600)], 32, 8), ([(2100, 2300), (1, 600)], 32, 8)],
+                         ids=["few rows", "many rows", "most rows"])
+def test_infinite_values_of_vanishing_weight(pairs, H, Hkv):
+    """A visible infinity in V whose weight is below f32's range, in this part of the keys or another: an infinity or NaN in its
+    dim, nothing elsewhere; the largest values that are sure to stay finite beside it."""
+    s = Setup(pairs, 16, H, Hkv, 128, "bf16", seed=25)
+    s.q[:, :H // Hkv, 0] = 8.0
+    s.k[0][:, 0, 0] = torch.linspace(0, 1600, pairs[0][1], device="cuda").bfloat16()
+    big = 2.0 ** 103
+    s.v[0][:, 1:, :] = s.v[0][:, 1:, :].clamp(-4, 4) * big              # 2^105 x 2^14 keys
+    s.v[0][1, 0, 5] = float("inf")
+    s.fill()
+    out, lse = s.attend()
+    mine = out[s.ends[0]:s.ends[1], :H // Hkv, 5]
+    assert not bool(torch.isfinite(mine).any())
+    out[s.ends[0]:s.ends[1], :H // Hkv, 5] = 0.0
+    s.v[0][:, 0, 5] = 0.0
+    s.compare(out, lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 def test_pages_beyond_4_gigabytes(fmt):
     """Requests whose pages lie at the end of a pool of more than 2^32 bytes and 2^31 elements."""

@@ -134,6 +134,62 @@ def test_rows_whose_logits_are_all_minus_infinity(lens, H, Hkv, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,Hkv", SIZES, ids=["32", "128", "256"])
+def test_values_up_to_the_end_of_the_range(lens, H, Hkv, D):
+    """v times a power of two, up to 2^120 / keys: the outputs times that power, bit for bit, while the maximum lags behind
+    climbing logits."""
+    q, k, v, cu = packed(lens, H, Hkv, D, seed=39)
+    n = max(lens)
+    ramp = torch.linspace(0, 1, q.shape[0], device="cuda")[:, None, None]
+    k = (k + 0.3 * q[:, :Hkv] * ramp).bfloat16()
+    v = v.clamp(-4, 4)
+    big = 2.0 ** (117 - math.ceil(math.log2(n)))
+    (out, lse), (far, same) = mp.prompt_attention(q, k, v, cu), mp.prompt_attention(q, k, v * big, cu)
+    compare(q, k, v, cu, out, lse)
+    assert bool(torch.isfinite(far).all()) and torch.equal(far.double(), out.double() * big) and torch.equal(same, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,Hkv", SIZES, ids=["32", "128", "256"])
+def test_logits_up_to_the_end_of_the_range(lens, H, Hkv, D):
+    """|scale q . k| up to 2^24, climbing and falling: finite, within the error of f32 logits."""
+    q, k, v, cu = packed(lens, H, Hkv, D, seed=41)
+    ramp = torch.linspace(0.1, 1, q.shape[0], device="cuda")[:, None, None]
+    for ks in ((k * ramp).bfloat16(), (k * ramp.flip(0)).bfloat16()):
+        top = max(float((q[:, h].float() @ ks[:, h * Hkv // H].float().t()).abs().max()) for h in range(H))
+        scale = 0.99 * 2.0 ** 24 / top
+        out, lse = mp.prompt_attention(q, ks, v, cu, scale=scale)
+        assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+        compare(q, ks, v, cu, out, lse, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,Hkv", SIZES, ids=["32", "128", "256"])
+def test_infinite_values_of_vanishing_weight(lens, H, Hkv, D):
+    """A visible infinity in V whose weight is below f32's range: an infinity or NaN in its dim, nothing elsewhere."""
+    q, k, v, cu = packed(lens, H, Hkv, D, seed=40)
+    a, b = int(cu[-2]), int(cu[-1])
+    q[a:, :H // Hkv, 0] = 8.0
+    k[a:b, 0, 0] = torch.linspace(0, 800, b - a, device="cuda").bfloat16()
+    v[a + 1, 0, 5], v[a + 70, 0, 6] = float("inf"), float("-inf")
+    out, lse = mp.prompt_attention(q, k, v, cu)
+    for dim, key in ((5, a + 1), (6, a + 70)):
+        group = out[:, :H // Hkv, dim]
+        assert not bool(torch.isfinite(group[key:b]).any()) and bool(torch.isfinite(group[:key]).all())
+        out[key:b, :H // Hkv, dim] = 0.0
+        v[key, 0, dim] = 0.0
+    keep = torch.ones(D, dtype=torch.bool, device="cuda")
+    keep[5] = keep[6] = False
+    for i, j in zip(cu.tolist(), cu.tolist()[1:]):
+        o, t, z, zt = attention64.attend(q[i:j], k[i:j], v[i:j], D ** -0.5, torch.arange(j - i))
+        attention64.check(out[i:j][..., keep], o[..., keep], t[..., keep])
+        attention64.check(lse[i:j], z, zt)
+
+
+@pytest.mark.gpu
 def test_peaked_and_flat_rows():
     """Logits of thousands next to zeros: the maximum moves far and late, weights underflow."""
     q, k, v, cu = packed([500], 4, 2, 128, seed=8)
