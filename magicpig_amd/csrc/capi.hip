@@ -1802,7 +1802,7 @@ int mp_paged_alloc(mp_paged_t* h, int num_layers, int num_attention_heads, int n
         rc = alloc_zero((void**)&h->pool[i], (size_t)(h->rows() * h->row_bytes()));
         if (rc == MP_OK && kv_format == MP_KV_E4M3) rc = alloc_zero((void**)&h->scale[i], (size_t)(h->rows() * 2));
     }
-    if (rc == MP_OK) rc = alloc_zero((void**)&h->err, 4);
+    if (rc == MP_OK) rc = alloc_zero((void**)&h->err, 2 * sizeof(int));
     if (rc == MP_OK && hipStreamSynchronize(nullptr) != hipSuccess)        // the zeros are there for calls on any stream
         rc = fail(MP_ERR_HIP, "mp_paged_alloc: clearing the pages failed");
     if (rc != MP_OK) { paged_free(h); return rc; }
@@ -1901,15 +1901,13 @@ int mp_paged_check(mp_paged_t* h, mp_stream_t stream) {
     MP_ON_DEVICE(h);
     MP_REQUIRE(h && h->allocated, MP_ERR_STATE, "mp_paged_check: not allocated");
     hipStream_t st = (hipStream_t)stream;
-    int flag = 0;
-    MP_HIP_CHECK(hipMemcpyAsync(&flag, h->err, 4, hipMemcpyDeviceToHost, st));
+    int flags = 0;
+    MP_HIP_CHECK(launch_paged_take_flags(h->err, st));
+    MP_HIP_CHECK(hipMemcpyAsync(&flags, h->err + 1, sizeof(int), hipMemcpyDeviceToHost, st));
     MP_HIP_CHECK(hipStreamSynchronize(st));
-    if (flag) {
-        MP_HIP_CHECK(hipMemsetAsync(h->err, 0, 4, st));
-        MP_HIP_CHECK(hipStreamSynchronize(st));
-        return fail(MP_ERR_DATA, flag & 1 ? "paged cache: a kv_len below 0 or beyond its page table"
-                                          : "paged cache: a page id outside the cache");
-    }
+    static const char* const met[] = {"", "a kv_len below 0 or beyond its page table", "a page id outside the cache",
+                                      "a kv_len below 0 or beyond its page table, and a page id outside the cache"};
+    MP_REQUIRE(flags == 0, MP_ERR_DATA, std::string("paged cache: ") + met[flags & 3]);
     return MP_OK;
 }
 

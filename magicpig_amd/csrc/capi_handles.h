@@ -147,7 +147,7 @@ struct mp_paged {
     bool allocated = false;
     char** pool = nullptr;         // per layer, see paged.hip
     uint8_t** scale = nullptr;     // per layer, null for MP_KV_BF16
-    int* err = nullptr;            // device: what the kernels met (1 = kv_len, 2 = page id)
+    int* err = nullptr;            // device: what the kernels met (1 = kv_len, 2 = page id), and what mp_paged_check took of it
     int64_t rows() const { return pages * Hkv << shift; }
     int64_t row_bytes() const { return 2 * (int64_t)D * (format == MP_KV_E4M3 ? 1 : 2); }
 };

@@ -80,6 +80,7 @@ hipError_t launch_paged_read(uint16_t*, uint16_t*, const int32_t*, int, int, con
 hipError_t launch_paged_attention(const uint16_t*, int64_t, int64_t, const int32_t*, int, int, const int32_t*, int,
                                   const int32_t*, int, int, int, int, int, bool, const char*, const uint8_t*, int*, float, int,
                                   uint16_t*, float*, char*, hipStream_t);
+hipError_t launch_paged_take_flags(int*, hipStream_t);
 bool lsh_hash_only_supported(int L);
 hipError_t launch_attn_ticket_check(int*, int, int*, hipStream_t);
 hipError_t launch_relay(const void*, void*, size_t, hipStream_t);

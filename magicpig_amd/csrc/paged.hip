@@ -619,7 +619,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     if (a.lse != nullptr && l == 0) a.lse[row] = log_sum(m, sum);
 }
 
+// What the kernels met since the last look: taken and cleared in one step, so that nothing that another stream reports meanwhile is lost.
+__global__ void paged_take_flags_kernel(int* err) { err[1] = atomicExch(err, 0); }
+
 // ---------------------------------------------------------------- host
+hipError_t launch_paged_take_flags(int* err, hipStream_t st) {
+    paged_take_flags_kernel<<<1, 1, 0, st>>>(err);
+    return hipGetLastError();
+}
+
 // Tokens a workgroup copies: one pass of its threads at least, and from 2048 tokens on up to 8, as long as that leaves a CU
 // eight workgroups (fewer lookups).
 static int copy_tokens(int64_t T, int Hkv, int D) {

@@ -457,6 +457,26 @@ def test_rows_past_the_table_are_skipped(more, D, fmt):
 
 
 @pytest.mark.gpu
+def test_check_names_all_that_was_met_and_forgets_it():
+    s = Setup([(1, 100), (2, 90)], 16, 8, 2, 128, "bf16", seed=19).fill()
+    t, n = s.table.clone(), s.kv_len.clone()
+    t[1, 0], n[0] = -1, 113
+    for _ in range(2):
+        s.cache.attention(0, s.q, s.cu, t, n)
+        with pytest.raises(mp.MagicPigError, match="kv_len.*page id"):
+            s.cache.check()
+        s.cache.check()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        s.cache.read(0, 3, s.cu, s.table, n)
+        with pytest.raises(mp.MagicPigError, match="kv_len"):
+            s.cache.check()
+    s.cache.check()
+    s.compare(*s.attend())
+
+
+@pytest.mark.gpu
 def test_no_new_rows():
     s = Setup([(0, 100), (0, 3)], 16, 8, 2, 128, "bf16").fill()
     out, lse = s.attend()
