@@ -16,7 +16,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from .prompt_attention import rows_strides, same_device
+from .prompt_attention import rows_strides, same_device, written
 
 
 class PagedKVCache:
@@ -78,8 +78,8 @@ class PagedKVCache:
             k = page_table.new_empty(shape, dtype=torch.bfloat16)
         if v is None:
             v = page_table.new_empty(shape, dtype=torch.bfloat16)
-        L.expect(k, torch.bfloat16, shape, "k")
-        L.expect(v, torch.bfloat16, shape, "v")
+        written(k, torch.bfloat16, shape, "k")
+        written(v, torch.bfloat16, shape, "v")
         same_device(self._device, k=k, v=v)
         L.check(L.lib().mp_paged_read(self._h, layer_id, k.data_ptr(), v.data_ptr(), *rows,
                                       L.stream_on(self._device)))
@@ -97,11 +97,11 @@ class PagedKVCache:
         if out is None:
             out = q.new_empty((T, H, D))
         else:
-            L.expect(out, torch.bfloat16, (T, H, D), "out")
+            written(out, torch.bfloat16, (T, H, D), "out")
         if lse is None:
             lse = q.new_empty((T, H), dtype=torch.float32)
         else:
-            L.expect(lse, torch.float32, (T, H), "lse")
+            written(lse, torch.float32, (T, H), "lse")
         rows = self._rows(T, cu_seqlens, page_table, kv_len, q=q, out=out, lse=lse)
         size = self._workspace(rows[1], T, rows[4])
         # from torch's allocator: safe to reuse in stream order, and a captured graph's own

@@ -4,8 +4,15 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
+
+
+def differentiated(t: torch.Tensor) -> bool:
+    """Whether autograd follows t, backwards or forwards (a tangent of an open dual level)."""
+    return (t.requires_grad and torch.is_grad_enabled()) or (
+        forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None)
 
 
 def rows_strides(t: torch.Tensor, heads: int, head_dim: int, name: str):
@@ -15,7 +22,7 @@ def rows_strides(t: torch.Tensor, heads: int, head_dim: int, name: str):
         n, h, d = t.shape
         if t.dtype is torch.bfloat16 and h == heads and d == head_dim and t.is_cuda:
             st, sh, sd = t.stride()
-            if sd == 1 and not (t.requires_grad and torch.is_grad_enabled()):
+            if sd == 1 and not differentiated(t):
                 return n, st if n > 1 else heads * head_dim, sh if heads > 1 else head_dim
     except (AttributeError, ValueError):
         pass
@@ -29,7 +36,14 @@ def rows_strides(t: torch.Tensor, heads: int, head_dim: int, name: str):
         raise ValueError(f"{name}: expected a CUDA tensor")
     if t.stride(2) != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    raise ValueError(f"{name}: requires a gradient, and there is no backward (torch.no_grad() for inference)")
+    raise ValueError(f"{name}: requires a gradient or has a tangent, and there is no backward (torch.no_grad() for inference)")
+
+
+def written(t: torch.Tensor, dtype, shape, name: str) -> None:
+    """Checks a contiguous tensor that a call is to fill."""
+    L.expect(t, dtype, shape, name)
+    if differentiated(t):
+        raise ValueError(f"{name}: requires a gradient or has a tangent, and there is no backward")
 
 
 def same_device(index: int, **tensors) -> None:
@@ -62,11 +76,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if out is None:
         out = q.new_empty((T, H, D))
     else:
-        L.expect(out, torch.bfloat16, (T, H, D), "out")
+        written(out, torch.bfloat16, (T, H, D), "out")
     if lse is None:
         lse = q.new_empty((T, H), dtype=torch.float32)
     else:
-        L.expect(lse, torch.float32, (T, H), "lse")
+        written(lse, torch.float32, (T, H), "lse")
     device = q.get_device()
     same_device(device, k=k, v=v, cu_seqlens=cu_seqlens, out=out, lse=lse)
     args = (q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, T,

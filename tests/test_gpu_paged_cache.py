@@ -518,6 +518,22 @@ def test_refusals_without_a_handle():
 
 
 @pytest.mark.gpu
+def test_forward_gradients_are_refused():
+    s = Setup([(2, 100)], 16, 8, 2, 128, "bf16").fill()
+    with torch.autograd.forward_ad.dual_level():
+        q, k = (torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)) for x in (s.q, s.k[0][:2]))
+        with pytest.raises(ValueError, match="q: .*tangent"):
+            s.cache.attention(0, q, s.cu, s.table, s.kv_len)
+        with pytest.raises(ValueError, match="v: .*tangent"):
+            s.cache.append(0, s.k[0][:2], k, s.cu, s.table, s.kv_len)
+    leaf = torch.empty((2, 2, 128), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="k: requires a gradient"):
+        s.cache.read(0, 2, s.cu, s.table, s.kv_len, k=leaf)
+    with pytest.raises(ValueError, match="out: requires a gradient"):
+        s.attend(out=torch.empty_like(s.q).requires_grad_())
+
+
+@pytest.mark.gpu
 def test_refusals_of_calls():
     s = Setup([(2, 100)], 16, 8, 2, 128, "bf16").fill()
     c, k, cu, t, n = s.cache, s.k[0][:2], s.cu, s.table, s.kv_len

@@ -296,6 +296,22 @@ def test_gradients_are_refused():
 
 
 @pytest.mark.gpu
+def test_forward_gradients_are_refused():
+    q, k, v, cu = packed([4], 8, 2, 128)
+    t = torch.ones_like(v)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(v, t)
+        with pytest.raises(ValueError, match="v: .*tangent"):
+            mp.prompt_attention(q, k, dual, cu)
+        mp.prompt_attention(q, k, v, cu)                   # an open level alone is no reason
+    with pytest.raises(ValueError, match="v: .*tangent"):
+        torch.func.jvp(lambda x: mp.prompt_attention(q, k, x, cu)[0], (v,), (t,))
+    for name, x in (("out", torch.empty_like(q)), ("lse", torch.empty((4, 8), device="cuda"))):
+        with pytest.raises(ValueError, match=name + ": requires a gradient"):
+            mp.prompt_attention(q, k, v, cu, **{name: x.requires_grad_()})
+
+
+@pytest.mark.gpu
 def test_empty_inputs():
     q, k, v, cu = packed([0, 0], 8, 2, 128)
     out, lse = mp.prompt_attention(q, k, v, cu)
