@@ -392,7 +392,8 @@ int mp_decode_layer_window_ex(mp_simhash_t* s, mp_lsh_t* lsh, mp_attn_t* attn, m
  *   fused projection are used in place; dims contiguous), every address 16-byte aligned, token strides below 2^23;
  *   cu_seqlens int32 [num_seqs + 1] (device): sequence b is the rows cu_seqlens[b] .. cu_seqlens[b + 1]; sequences may be
  *   empty; rows in front of the first and behind the last sequence are not read and their outputs stay as they were;
- *   output bf16 [num_tokens, H, D], lse f32 [num_tokens, H] (base-2 log-sum-exp, may be NULL), contiguous.
+ *   output bf16 [num_tokens, H, D], lse f32 [num_tokens, H] (base-2 log-sum-exp, may be NULL), contiguous; they overlap neither
+ *   an input nor each other, except that output may be q itself (the same contiguous rows).
  * Token i of a sequence sees its tokens 0 .. i; query head h reads kv head h / (H / Hkv).  head_dim 64 or 128; scale > 0.
  * Logits, weights' sums and outputs are summed in f32; the weights are rounded to bf16 for the product with V, so an output is off
  * by up to 2^-8 of sum |weight v| and 2^-8 of itself (its own rounding).  Finite inputs give finite results while every
@@ -436,12 +437,14 @@ int mp_paged_append(mp_paged_t* h, int layer_id, const uint16_t* k, int64_t k_to
                     const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens, int num_seqs,
                     int64_t num_tokens, const int32_t* page_table, int pages_per_seq, const int32_t* kv_len,
                     mp_stream_t stream);
-/* The inverse: the same rows out of the pages, bf16 [num_tokens, Hkv, D] (MP_KV_E4M3: what the codes stand for). */
+/* The inverse: the same rows out of the pages, bf16 [num_tokens, Hkv, D] (MP_KV_E4M3: what the codes stand for); k and v do not
+ * overlap. */
 int mp_paged_read(mp_paged_t* h, int layer_id, uint16_t* k, uint16_t* v, const int32_t* cu_seqlens, int num_seqs,
                   int64_t num_tokens, const int32_t* page_table, int pages_per_seq, const int32_t* kv_len,
                   mp_stream_t stream);
 /* New row i of request b attends to the request's positions 0 .. kv_len[b] - n_b + i as the cache holds them.
- * q [num_tokens, H, D]; output bf16 [num_tokens, H, D]; lse f32 [num_tokens, H] (base 2, may be NULL); scale > 0.
+ * q [num_tokens, H, D]; output bf16 [num_tokens, H, D]; lse f32 [num_tokens, H] (base 2, may be NULL); scale > 0.  Output, lse
+ * and workspace overlap neither q nor each other, except that output may be q itself (the same contiguous rows).
  * workspace: at least mp_paged_workspace(...) bytes, 16-byte aligned, not shared with a call that may run at the same time
  * (may be NULL where that is 0); its contents need no preparation.  The keys of a row are split over workgroups when the
  * rows are few, and joined in a fixed order: results do not vary from run to run.  Precision, range and what infinities and NaN

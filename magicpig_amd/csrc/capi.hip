@@ -1719,6 +1719,31 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 static bool row_strides_ok(int64_t token, int64_t head) {
     return token >= 0 && head >= 0 && token % 8 == 0 && head % 8 == 0 && token < (1 << 23);
 }
+// whether rows [tokens, heads, D] of 16 bits at `rows` and `bytes` at `block` share memory (along the
+// larger stride each piece counts by itself, a gap inside a piece as part of it)
+static bool touches(const void* rows, int64_t tokens, int64_t heads, int D, int64_t token, int64_t head, const void* block, int64_t bytes) {
+    typedef __int128 wide;                                          // (strides may be anything)
+    const bool by_token = token >= head;
+    const wide outer = (wide)(by_token ? token : head) * 2, inner = (wide)(by_token ? head : token) * 2;
+    const wide n = by_token ? tokens : heads, m = by_token ? heads : tokens, extent = (m - 1) * inner + D * 2;
+    const wide first = (wide)reinterpret_cast<uintptr_t>(rows), lo = (wide)reinterpret_cast<uintptr_t>(block), hi = lo + bytes;
+    if (first >= hi) return false;
+    wide last = outer == 0 ? 0 : (hi - 1 - first) / outer;          // the last of n pieces that begins in front of hi
+    if (last > n - 1) last = n - 1;
+    return first + last * outer + extent > lo;
+}
+static bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y ? y - x < (uintptr_t)a_bytes : x - y < (uintptr_t)b_bytes;
+}
+// What attention writes -- output [T, H, D], lse [T, H] -- lies apart from its queries, or the output is these very rows: a
+// workgroup writes the rows it read, when it has read them.
+static bool outputs_apart(const uint16_t* q, int64_t token, int64_t head, int64_t T, int H, int D, const uint16_t* output, const float* lse) {
+    const int64_t out_bytes = T * H * D * 2, lse_bytes = T * H * 4;
+    const bool same = q == output && (T == 1 || token == (int64_t)H * D) && (H == 1 || head == D);
+    return (same || !touches(q, T, H, D, token, head, output, out_bytes)) &&
+           (!lse || (!touches(q, T, H, D, token, head, lse, lse_bytes) && !overlap(output, out_bytes, lse, lse_bytes)));
+}
 static bool attention_scale_ok(float scale) { return scale > 0.f && scale < __builtin_inff(); }
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -1741,6 +1766,13 @@ int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_hea
                "mp_prompt_attention: q, k, v and output must be 16-byte aligned");
     MP_REQUIRE(num_tokens <= (1ll << 30) / (H / Hkv) && prompt_threads(num_tokens, num_seqs, H, Hkv, head_dim) < 1ll << 32,
                MP_ERR_UNSUPPORTED, "mp_prompt_attention: more rows than one launch can number");
+    const int64_t out_bytes = num_tokens * H * head_dim * 2, lse_bytes = lse ? num_tokens * H * 4 : 0;
+    MP_REQUIRE(outputs_apart(q, q_token_stride, q_head_stride, num_tokens, H, head_dim, output, lse) &&
+                   !touches(k, num_tokens, Hkv, head_dim, k_token_stride, k_head_stride, output, out_bytes) &&
+                   !touches(v, num_tokens, Hkv, head_dim, v_token_stride, v_head_stride, output, out_bytes) &&
+                   (!lse || (!touches(k, num_tokens, Hkv, head_dim, k_token_stride, k_head_stride, lse, lse_bytes) &&
+                             !touches(v, num_tokens, Hkv, head_dim, v_token_stride, v_head_stride, lse, lse_bytes))),
+               MP_ERR_INVALID, "mp_prompt_attention: output and lse must not overlap the inputs or each other");
     MP_HIP_CHECK(launch_prompt_attention(q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, v,
                                          v_token_stride, v_head_stride, cu_seqlens, num_seqs, (int)num_tokens, H, Hkv,
                                          head_dim, scale * LOG2E, output, lse, (hipStream_t)stream));
@@ -1856,6 +1888,8 @@ int mp_paged_read(mp_paged_t* h, int layer_id, uint16_t* k, uint16_t* v, const i
     if (num_tokens == 0) return MP_OK;
     MP_REQUIRE(k && v, MP_ERR_INVALID, "mp_paged_read: null argument");
     MP_REQUIRE(aligned16(k) && aligned16(v), MP_ERR_INVALID, "mp_paged_read: k and v must be 16-byte aligned");
+    const int64_t bytes = num_tokens * h->Hkv * h->D * 2;
+    MP_REQUIRE(!overlap(k, bytes, v, bytes), MP_ERR_INVALID, "mp_paged_read: k and v must not overlap");
     MP_HIP_CHECK(launch_paged_read(k, v, cu_seqlens, num_seqs, (int)num_tokens, page_table, pages_per_seq, kv_len, h->shift,
                                    (int)h->pages, h->Hkv, h->D, h->format == MP_KV_E4M3, h->pool[layer_id], h->scale[layer_id],
                                    h->err, (hipStream_t)stream));
@@ -1890,6 +1924,11 @@ int mp_paged_attention(mp_paged_t* h, int layer_id, const uint16_t* q, int64_t q
     const int64_t need = paged_workspace_bytes(num_tokens, num_seqs, h->H, h->Hkv, h->D, capacity, h->cus);
     MP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), MP_ERR_INVALID,
                "mp_paged_attention: workspace smaller than mp_paged_workspace says, or not 16-byte aligned");
+    const int64_t out_bytes = num_tokens * h->H * h->D * 2, lse_bytes = num_tokens * h->H * 4;
+    MP_REQUIRE(outputs_apart(q, q_token_stride, q_head_stride, num_tokens, h->H, h->D, output, lse) &&
+                   (need == 0 || (!touches(q, num_tokens, h->H, h->D, q_token_stride, q_head_stride, workspace, need) &&
+                                  !overlap(output, out_bytes, workspace, need) && !(lse && overlap(lse, lse_bytes, workspace, need)))),
+               MP_ERR_INVALID, "mp_paged_attention: output, lse and workspace must not overlap the queries or each other");
     MP_HIP_CHECK(launch_paged_attention(q, q_token_stride, q_head_stride, cu_seqlens, num_seqs, (int)num_tokens, page_table,
                                         pages_per_seq, kv_len, h->shift, (int)h->pages, h->H, h->Hkv, h->D,
                                         h->format == MP_KV_E4M3, h->pool[layer_id], h->scale[layer_id], h->err, scale * LOG2E,

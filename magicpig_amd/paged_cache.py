@@ -90,7 +90,8 @@ class PagedKVCache:
                   lse: torch.Tensor | None = None):
         """q bf16 [T, H, D]: row cu_seqlens[b] + i attends to positions 0 .. kv_len[b] - n_b + i of request b, as the pages hold
         them (append the rows' own keys first); query head h to kv head h // (H // Hkv).  Returns (out bf16 [T, H, D],
-        lse f32 [T, H], base 2); a row that sees nothing gives 0 and -inf.  scale: default head_dim ** -0.5.  Sums are f32, the
+        lse f32 [T, H], base 2); a row that sees nothing gives 0 and -inf.  scale: default head_dim ** -0.5.  `out` may be q itself (any
+        other overlap is refused).  Sums are f32, the
         weights are rounded to bf16 for the product with v."""
         H, D = self.H, self.D
         T, qt, qh = rows_strides(q, H, D, "q")

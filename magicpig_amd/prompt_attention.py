@@ -58,7 +58,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     fused projection go in as they are); cu_seqlens int32 [B + 1]: sequence b is the rows cu_seqlens[b] .. cu_seqlens[b + 1].
     Returns (out bf16 [T, H, D], lse f32 [T, H], base 2): token i of a sequence attends to its tokens 0 .. i, query head h to
     kv head h // (H // Hkv).  scale: default head_dim ** -0.5.  Rows outside every sequence are not written: give `out` /
-    `lse` where their contents matter.  head_dim 64 or 128.  Sums are f32, the weights are rounded to bf16 for the product with v.
+    `lse` where their contents matter (`out` may be q itself; any other overlap is refused).  head_dim 64 or 128.  Sums are f32, the weights are rounded to bf16 for the product with v.
     Runs on torch's current stream of q's device."""
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise ValueError("q: expected a tensor [tokens, heads, head_dim]")

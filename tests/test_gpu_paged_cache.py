@@ -518,6 +518,25 @@ def test_refusals_without_a_handle():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pairs,H,Hkv", [([(1, 9000), (5, 700)], 8, 2), ([(300, 4000), (1, 600)], 32, 8), ([(2100, 2300), (1, 600)], 32, 8)],
+                         ids=["few rows", "many rows", "most rows"])
+def test_outputs_over_the_queries(pairs, H, Hkv):
+    s = Setup(pairs, 16, H, Hkv, 128, "bf16", seed=26).fill()
+    want = s.attend()
+    out, lse = s.cache.attention(0, s.q, s.cu, s.table, s.kv_len, out=s.q)
+    assert out is s.q and torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    room = torch.zeros(s.q.numel() + 64, dtype=torch.bfloat16, device="cuda")
+    a, b = (room[i:i + s.q.numel()].view_as(s.q) for i in (0, 64))
+    with pytest.raises(mp.MagicPigError, match="overlap"):
+        s.cache.attention(0, a, s.cu, s.table, s.kv_len, out=b)
+    with pytest.raises(mp.MagicPigError, match="overlap"):
+        s.cache.attention(0, s.q, s.cu, s.table, s.kv_len, out=a, lse=room.view(torch.float32)[:s.T * H].view(s.T, H))
+    k = torch.zeros((s.T, Hkv, 128), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(mp.MagicPigError, match="overlap"):
+        s.cache.read(0, s.T, s.cu, s.table, s.kv_len, k=k, v=k)
+
+
+@pytest.mark.gpu
 def test_forward_gradients_are_refused():
     s = Setup([(2, 100)], 16, 8, 2, 128, "bf16").fill()
     with torch.autograd.forward_ad.dual_level():

@@ -312,6 +312,34 @@ def test_forward_gradients_are_refused():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,H,Hkv", SIZES, ids=["32", "128", "256"])
+def test_outputs_beside_inputs_and_over_the_queries(lens, H, Hkv, D):
+    q, k, v, cu = packed(lens, H, Hkv, D, seed=42)
+    want = mp.prompt_attention(q, k, v, cu)
+    T = q.shape[0]
+    room = torch.zeros(T * (2 * H + 2 * Hkv) * D, dtype=torch.bfloat16, device="cuda")       # all four, one behind the other
+    qq, oo, kk, vv = (x.view(T, -1, D) for x in room.split([T * H * D, T * H * D, T * Hkv * D, T * Hkv * D]))
+    for x, y in ((qq, q), (kk, k), (vv, v)):
+        x.copy_(y)
+    got = mp.prompt_attention(qq, kk, vv, cu, out=oo)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    got = mp.prompt_attention(qq, kk, vv, cu, out=qq)
+    assert got[0] is qq and torch.equal(qq, want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(mp.MagicPigError, match="overlap"):
+        mp.prompt_attention(oo, kk, vv, cu, out=room[8:T * H * D + 8].view(T, H, D))
+
+
+@pytest.mark.gpu
+def test_one_token_in_one_fused_row():
+    """q, k, v and the output side by side in one row."""
+    q, k, v, cu = packed([1], 8, 2, 128, seed=43)
+    row = torch.cat([q, k, v, torch.zeros_like(q)], dim=1)
+    out, _ = mp.prompt_attention(row[:, :8], row[:, 8:10], row[:, 10:12], cu, out=row[:, 12:])
+    assert torch.equal(out, v.repeat_interleave(4, 1)) and torch.equal(row[:, 12:], out)
+
+
+@pytest.mark.gpu
 def test_empty_inputs():
     q, k, v, cu = packed([0, 0], 8, 2, 128)
     out, lse = mp.prompt_attention(q, k, v, cu)
@@ -346,6 +374,22 @@ def test_refusals_of_the_c_entry(change, code):
     a = {**GOOD, **change}
     assert L.lib().mp_prompt_attention(*(a[n] for n in GOOD)) == code
     assert b"mp_prompt_attention" in L.lib().mp_last_error()
+
+
+BASE, T, ROW = 1 << 24, 10, 128 * 2          # 10 tokens; bytes of a head's row
+
+
+@pytest.mark.parametrize("change", [
+    dict(out=BASE, k=BASE + 8 * ROW), dict(out=BASE, k=BASE + T * 8 * ROW - 16), dict(out=BASE, v=BASE - T * 2 * ROW + 16),
+    dict(out=BASE, q=BASE + 16), dict(out=BASE, q=BASE, qt=2048), dict(out=BASE, q=BASE, qh=T * 128, qt=128), dict(out=BASE, q=BASE - T * 8 * ROW + 16),
+    dict(out=BASE, lse=BASE + T * 8 * ROW - 4), dict(out=BASE, lse=BASE - 4), dict(lse=BASE, q=BASE), dict(lse=BASE, k=BASE - T * 2 * ROW + 16),
+    dict(lse=BASE, v=BASE + T * 8 * 4 - 16), dict(out=BASE, k=BASE - 9 * 8192 * 2, kt=8192), dict(out=1 << 45, v=1 << 44, vh=1 << 43, vt=1 << 20),
+    dict(out=BASE, k=BASE, kt=0, kh=0), dict(out=BASE, k=BASE - (1 << 20), kh=(1 << 62) + (1 << 61), kt=(1 << 23) - 8)])
+def test_outputs_over_inputs_are_refused(change):
+    far = dict(q=1 << 40, k=2 << 40, v=3 << 40, out=4 << 40, lse=5 << 40)
+    a = {**GOOD, "tokens": T, **far, **change}
+    assert L.lib().mp_prompt_attention(*(a[n] for n in GOOD)) == 1
+    assert b"overlap" in L.lib().mp_last_error()
 
 
 def test_refusals_of_the_python_entry():
