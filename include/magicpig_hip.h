@@ -394,7 +394,7 @@ int mp_decode_layer_window_ex(mp_simhash_t* s, mp_lsh_t* lsh, mp_attn_t* attn, m
  *   empty; rows in front of the first and behind the last sequence are not read and their outputs stay as they were;
  *   output bf16 [num_tokens, H, D], lse f32 [num_tokens, H] (base-2 log-sum-exp, may be NULL), contiguous; they overlap neither
  *   an input nor each other, except that output may be q itself (the same contiguous rows).
- * Token i of a sequence sees its tokens 0 .. i; query head h reads kv head h / (H / Hkv).  head_dim 64 or 128; scale > 0.
+ * Token i of a sequence sees its tokens 0 .. i; query head h reads kv head h / (H / Hkv).  head_dim 64 or 128; 0 < scale < 2^127.
  * Logits, weights' sums and outputs are summed in f32; the weights are rounded to bf16 for the product with V, so an output is off
  * by up to 2^-8 of sum |weight v| and 2^-8 of itself (its own rounding).  Finite inputs give finite results while every
  * |scale q . k| is below 2^24 and every |v| below 2^120 / (tokens the row sees).  An infinity or NaN in a key or value reaches the
@@ -443,7 +443,7 @@ int mp_paged_read(mp_paged_t* h, int layer_id, uint16_t* k, uint16_t* v, const i
                   int64_t num_tokens, const int32_t* page_table, int pages_per_seq, const int32_t* kv_len,
                   mp_stream_t stream);
 /* New row i of request b attends to the request's positions 0 .. kv_len[b] - n_b + i as the cache holds them.
- * q [num_tokens, H, D]; output bf16 [num_tokens, H, D]; lse f32 [num_tokens, H] (base 2, may be NULL); scale > 0.  Output, lse
+ * q [num_tokens, H, D]; output bf16 [num_tokens, H, D]; lse f32 [num_tokens, H] (base 2, may be NULL); 0 < scale < 2^127.  Output, lse
  * and workspace overlap neither q nor each other, except that output may be q itself (the same contiguous rows).
  * workspace: at least mp_paged_workspace(...) bytes, 16-byte aligned, not shared with a call that may run at the same time
  * (may be NULL where that is 0); its contents need no preparation.  The keys of a row are split over workgroups when the

@@ -1744,8 +1744,8 @@ static bool outputs_apart(const uint16_t* q, int64_t token, int64_t head, int64_
     return (same || !touches(q, T, H, D, token, head, output, out_bytes)) &&
            (!lse || (!touches(q, T, H, D, token, head, lse, lse_bytes) && !overlap(output, out_bytes, lse, lse_bytes)));
 }
-static bool attention_scale_ok(float scale) { return scale > 0.f && scale < __builtin_inff(); }
 constexpr float LOG2E = 1.4426950408889634f;
+static bool attention_scale_ok(float scale) { return scale > 0.f && scale * LOG2E < __builtin_inff(); }     // (the kernels' logits are base 2)
 
 int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
                         int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v, int64_t v_token_stride,
@@ -1756,7 +1756,7 @@ int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_hea
     MP_REQUIRE(head_dim == 64 || head_dim == 128, MP_ERR_UNSUPPORTED, "mp_prompt_attention: head_dim must be 64 or 128");
     MP_REQUIRE(Hkv >= 1 && H >= Hkv && H % Hkv == 0, MP_ERR_INVALID, "mp_prompt_attention: bad head counts");
     MP_REQUIRE(num_seqs >= 1 && num_tokens >= 0, MP_ERR_INVALID, "mp_prompt_attention: bad sequence or token count");
-    MP_REQUIRE(attention_scale_ok(scale), MP_ERR_INVALID, "mp_prompt_attention: scale must be finite and above 0");
+    MP_REQUIRE(attention_scale_ok(scale), MP_ERR_INVALID, "mp_prompt_attention: scale must be above 0, and finite in base 2");
     if (num_tokens == 0) return MP_OK;
     MP_REQUIRE(q && k && v && cu_seqlens && output, MP_ERR_INVALID, "mp_prompt_attention: null argument");
     MP_REQUIRE(row_strides_ok(q_token_stride, q_head_stride) && row_strides_ok(k_token_stride, k_head_stride) &&
@@ -1911,7 +1911,7 @@ int mp_paged_attention(mp_paged_t* h, int layer_id, const uint16_t* q, int64_t q
     MP_ON_DEVICE(h);
     if (int rc = paged_rows_check(h, layer_id, cu_seqlens, num_seqs, num_tokens, page_table, pages_per_seq, kv_len, "mp_paged_attention"))
         return rc;
-    MP_REQUIRE(attention_scale_ok(scale), MP_ERR_INVALID, "mp_paged_attention: scale must be finite and above 0");
+    MP_REQUIRE(attention_scale_ok(scale), MP_ERR_INVALID, "mp_paged_attention: scale must be above 0, and finite in base 2");
     if (num_tokens == 0) return MP_OK;
     MP_REQUIRE(q && output, MP_ERR_INVALID, "mp_paged_attention: null argument");
     MP_REQUIRE(row_strides_ok(q_token_stride, q_head_stride), MP_ERR_INVALID,

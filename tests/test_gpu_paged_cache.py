@@ -537,6 +537,14 @@ def test_outputs_over_the_queries(pairs, H, Hkv):
 
 
 @pytest.mark.gpu
+def test_a_scale_that_is_infinite_in_base_2_is_refused():
+    s = Setup([(2, 100)], 16, 8, 2, 128, "bf16").fill()
+    with pytest.raises(mp.MagicPigError, match="scale"):
+        s.attend(scale=3e38)
+    s.compare(*s.attend(scale=1e-20), scale=1e-20)
+
+
+@pytest.mark.gpu
 def test_forward_gradients_are_refused():
     s = Setup([(2, 100)], 16, 8, 2, 128, "bf16").fill()
     with torch.autograd.forward_ad.dual_level():

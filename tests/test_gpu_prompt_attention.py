@@ -376,6 +376,13 @@ def test_refusals_of_the_c_entry(change, code):
     assert b"mp_prompt_attention" in L.lib().mp_last_error()
 
 
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_a_scale_that_is_infinite_in_base_2_is_refused(scale):
+    far = dict(q=1 << 40, k=2 << 40, v=3 << 40, out=4 << 40, lse=5 << 40)
+    assert L.lib().mp_prompt_attention(*({**GOOD, **far, "scale": scale, "tokens": 0}[n] for n in GOOD)) == 1
+    assert b"scale" in L.lib().mp_last_error()
+
+
 BASE, T, ROW = 1 << 24, 10, 128 * 2          # 10 tokens; bytes of a head's row
 
 
