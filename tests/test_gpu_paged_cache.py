@@ -179,6 +179,46 @@ def test_workgroups_of_many_rows_whole_and_in_parts(pairs, H, Hkv, D, fmt):
     s.compare(*s.attend())
 
 
+def workspace(s):
+    need = C.c_int64()
+    L.check(L.lib().mp_paged_workspace(s.cache._h, len(s.pairs), s.T, s.table.shape[1], C.byref(need)))
+    return need.value
+
+
+# 128 rows a workgroup: tables of at most 512 positions and more rows than the kernel for few of them takes; 256 at head_dim 128
+# and 2^16 rows; rows enough to fill the chip behind longer tables
+UNCUT = [([(300, 500), (17, 512), (0, 40), (90, 90), (257, 300), (60, 20)], 32, 8), ([(500, 512), (1, 3), (511, 511), (400, 100)] * 2, 32, 8),
+         ([(3000, 3500), (2500, 2500), (0, 9), (2700, 2900), (1, 700)], 32, 8)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("pairs,H,Hkv", UNCUT, ids=["short tables", "short tables, most rows", "a full chip"])
+def test_many_rows_whose_keys_are_not_cut(pairs, H, Hkv, D, fmt):
+    """A workgroup finds its tile among the requests' slots, from the last one on."""
+    s = Setup(pairs, 32, H, Hkv, D, fmt, seed=27, before=3, behind=70).fill()
+    assert workspace(s) == 0
+    out, lse = torch.full_like(s.q, 7.0), torch.full((s.T, H), -3.0, device="cuda")
+    s.attend(out=out, lse=lse)
+    s.compare(out, lse)
+    for rows in (slice(0, 3), slice(s.ends[-1], s.T)):
+        assert bool((out[rows] == 7.0).all()) and bool((lse[rows] == -3.0).all())
+
+
+@pytest.mark.gpu
+def test_uncut_keys_and_offsets_that_are_none():
+    pairs, H, Hkv = UNCUT[0]
+    s = Setup(pairs, 32, H, Hkv, 128, "bf16", seed=28).fill()
+    T = s.T
+    for offsets in ([0, T, 1, 2, 3, 4, 5], [-9, T // 2, T + 70, 0, T, T, T], [T, 0, 0, T, 0, T, 0]):
+        cu = torch.tensor(offsets, dtype=torch.int32).cuda()
+        whole, sums = torch.full((T + 60, H, 128), 7.0, device="cuda", dtype=torch.bfloat16), torch.full((T + 60, H), -3.0, device="cuda")
+        s.cache.attention(0, s.q, cu, s.table, s.kv_len.clamp(max=500), out=whole[30:T + 30], lse=sums[30:T + 30])
+        for x, value in ((whole, 7.0), (sums, -3.0)):
+            assert bool((x[:30] == value).all()) and bool((x[T + 30:] == value).all())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 @pytest.mark.parametrize("pairs,H,Hkv", [([(30, 100), (1, 600)], 8, 2), ([(300, 4000), (1, 600)], 32, 8), ([(2100, 2300), (1, 600)], 32, 8)],
