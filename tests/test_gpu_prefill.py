@@ -3,7 +3,9 @@ a paged cache, run together as a server would: prefill, decode steps, captured g
 import pytest
 import torch
 
+import attention64
 from magicpig_amd import decode_harness as dh
+from test_gpu_paged_cache import stored
 
 SHAPE = dict(num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2, intermediate_size=768, vocab_size=1000)
 # A layer rounds its activations to bf16 at most 14 times between its input and output (norms, projections, rotation, attention
@@ -146,3 +148,115 @@ def test_refusals():
 def test_unknown_dense_cache_is_refused():
     with pytest.raises(ValueError, match="dense_cache"):
         dh.SyntheticLlamaDecoder(dense_cache="int4")
+
+
+# ---------------------------------------------------------------- layer by layer: attention to its own roundings
+def record(dec):
+    """Everything that passes through the decoder's attention: prompt layers (layer, hidden, q, k, v, out, hidden out), rows that
+    enter the state (layer, request): (k, v), dense decode layers (layer, q, k, v, out)."""
+    log, rows, steps = [], {}, []
+    layer_of, store, dense = dec._prompt_layer, dec._store_prompt, dec._dense_attention
+
+    def prompt_layer(layer, hidden, pos, attend):
+        kept = []
+
+        def watched(q, k, v):
+            out = attend(q, k, v)
+            kept.extend(x.clone() for x in (q, k, v, out))
+            return out
+        after = layer_of(layer, hidden, pos, watched)
+        log.append((layer, hidden.clone(), *kept, after.clone()))
+        return after
+
+    def store_prompt(layer, r, k, v):
+        rows[layer, r] = k.clone(), v.clone()
+        store(layer, r, k, v)
+
+    def dense_attention(q, k, v, layer):
+        out = dense(q, k, v, layer)
+        steps.append((layer, *(x.clone() for x in (q, k, v, out))))
+        return out
+    dec._prompt_layer, dec._store_prompt, dec._dense_attention = prompt_layer, store_prompt, dense_attention
+    return log, rows, steps
+
+
+def attention_is(out, q, k, v, first):
+    """`out` is the attention of q, whose row i sees keys 0 .. first + i, to its roundings; an output of zeros would not be."""
+    o, tol, _, _ = attention64.attend(q, k, v, q.shape[2] ** -0.5, torch.arange(q.shape[0]) + first)
+    attention64.check(out.view(o.shape), o, tol)
+    with pytest.raises(AssertionError, match="off by"):
+        attention64.check(torch.zeros_like(o), o, tol)
+
+
+# Roundings of a layer's hidden state behind the attention's output: 10 (output projection, sum, norm, gate and up, silu, their
+# product, down projection, sum; two more for what torch's products round inside), each by 2^-8 at most
+LAYER = 10 * 2.0 ** -8
+
+
+def layer_is(dec, layer, hidden, attn, after):
+    """The rest of the layer in f32 from the attention's own output; from an output of zeros it would be another."""
+    W, eps = dec.layers[layer], dec.shape.rms_norm_eps
+
+    def rest(a):
+        h = hidden.float() + a.reshape(hidden.shape[0], -1).float() @ W["wo"].float().t()
+        y = h / torch.sqrt((h * h).mean(-1, keepdim=True) + eps) * W["ln2"].float()
+        return h + (torch.nn.functional.silu(y @ W["gate"].float().t()) * (y @ W["up"].float().t())) @ W["down"].float().t()
+    want = rest(attn)
+    close(after, want, bound=LAYER)
+    with pytest.raises(AssertionError, match="differ"):
+        close(after, rest(torch.zeros_like(attn)), bound=LAYER)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_every_layer_of_a_packed_prefill(head_dim):
+    dec = decoder(head_dim)
+    log, rows, _ = record(dec)
+    lens = (400, 130)
+    dec.prefill(prompts(*lens))
+    assert [x[0] for x in log] == [0, 1, 2]
+    for layer, hidden, q, k, v, out, after in log:
+        for r, (a, b) in enumerate(((0, 400), (400, 530))):
+            attention_is(out[a:b], q[a:b], k[a:b], v[a:b], 0)
+            assert torch.equal(rows[layer, r][0], k[a:b]) and torch.equal(rows[layer, r][1], v[a:b])
+        layer_is(dec, layer, hidden, out, after)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunk", [150, 97])
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_every_layer_of_a_chunked_prefill(fmt, chunk):
+    """Each chunk's attention is over the rows as the cache's format holds them, and these are the rows the state gets."""
+    dec = decoder(dense_cache="bf16")
+    log, rows, _ = record(dec)
+    dec.prefill_chunked(1, prompts(400)[0], chunk=chunk, kv_format=fmt)
+    for layer in range(3):
+        mine = [x for x in log if x[0] == layer]
+        k, v = (stored(torch.cat([x[i] for x in mine]), fmt) for i in (3, 4))
+        assert [x[2].shape[0] for x in mine] == [min(chunk, 400 - i) for i in range(0, 400, chunk)]
+        for i, (_, hidden, q, _, _, out, after) in enumerate(mine):
+            seen = i * chunk + q.shape[0]
+            attention_is(out, q, k[:seen], v[:seen], i * chunk)
+            layer_is(dec, layer, hidden, out, after)
+        assert all(torch.equal(got.double(), want) for got, want in zip(rows[layer, 1], (k, v)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+def test_every_dense_layer_of_decode_steps_over_pages(fmt):
+    """Steps behind two prompts: each dense layer's attention is over the prompt's and the steps' rows as the pages hold them."""
+    dec = decoder(dense_layers=(0, 2), dense_cache=fmt)
+    _, rows, steps = record(dec)
+    lens = (400, 130)
+    ids = dec.prefill(prompts(*lens)).argmax(-1, keepdim=True)
+    for step in range(3):
+        ids = dec.inference(ids, torch.tensor([[n + step] for n in lens], device="cuda"))[:, -1].argmax(-1, keepdim=True)
+    dec.dense_server.check()
+    for layer in (0, 2):
+        mine = [x for x in steps if x[0] == layer]
+        assert len(mine) == 3
+        for r, n in enumerate(lens):
+            k, v = rows[layer, r]
+            for step, (_, q, kn, vn, out) in enumerate(mine):
+                k, v = torch.cat([k, kn[r].view(1, 2, -1)]), torch.cat([v, vn[r].view(1, 2, -1)])
+                attention_is(out[r], q[r].view(1, 4, -1), stored(k, fmt), stored(v, fmt), n + step)
