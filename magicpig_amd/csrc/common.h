@@ -19,9 +19,11 @@ int fail(int code, const std::string& msg);
 #define MP_HIP_CHECK(expr)                                                                  \
     do {                                                                                    \
         hipError_t _e = (expr);                                                             \
-        if (_e != hipSuccess)                                                               \
+        if (_e != hipSuccess) {                                                             \
+            (void)hipGetLastError(); /* reported here: not again by the thread's next launch */ \
             return ::mp::fail(_e == hipErrorOutOfMemory ? MP_ERR_NOMEM : MP_ERR_HIP,        \
                               std::string(#expr) + ": " + hipGetErrorString(_e));           \
+        }                                                                                   \
     } while (0)
 
 #define MP_REQUIRE(cond, code, msg)                      \

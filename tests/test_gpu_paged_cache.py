@@ -280,6 +280,28 @@ def test_infinite_values_of_vanishing_weight(pairs, H, Hkv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt,layers", [("bf16", 1), ("e4m3", 3)])
+def test_more_pages_than_the_memory_holds(fmt, layers):
+    """The allocation fails, gives back what it had, and leaves nothing behind for the calls after it."""
+    cache = mp.PagedKVCache()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    rows = int(0.4 * torch.cuda.mem_get_info()[1] / 256) if layers > 1 else (1 << 32) // 2       # the third layer, or the first, does not fit
+    with pytest.raises(mp.MagicPigError, match="MP_ERR_NOMEM"):
+        cache.alloc(layers, 8, 1, 128, rows // 4096, 4096, kv_format=fmt)
+    assert torch.equal(torch.arange(5, device="cuda") + 1, torch.arange(1, 6, device="cuda"))
+    assert torch.cuda.mem_get_info()[0] > free - (1 << 30)
+    with pytest.raises(mp.MagicPigError, match="not allocated"):
+        L.check(L.lib().mp_paged_check(cache._h, None))
+    cache.alloc(1, 8, 1, 128, 4, 64, kv_format=fmt)
+    k = torch.randn((3, 1, 128), device="cuda").bfloat16()
+    cu, table, n = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 3], [[2]], [3]))
+    cache.append(0, k, k, cu, table, n)
+    assert torch.equal(cache.read(0, 3, cu, table, n)[0].double(), stored(k, fmt))
+    cache.check()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
 def test_pages_beyond_4_gigabytes(fmt):
     """Requests whose pages lie at the end of a pool of more than 2^32 bytes and 2^31 elements."""
