@@ -399,7 +399,8 @@ int mp_decode_layer_window_ex(mp_simhash_t* s, mp_lsh_t* lsh, mp_attn_t* attn, m
  * by up to 2^-8 of sum |weight v| and 2^-8 of itself (its own rounding).  Finite inputs give finite results while every
  * |scale q . k| is below 2^24 and every |v| below 2^120 / (tokens the row sees).  An infinity or NaN in a key or value reaches the
  * rows that see it and no others: an infinity in V comes out as an infinity, or as NaN where its weight is too small for f32
- * (0 * inf); a row all of whose logits are -inf gives NaN and a log-sum-exp of -inf, as 0 / 0 does.  Offsets that decrease or leave [0, num_tokens] are clamped (no access outside the tensors), the results are then unspecified.  Device pointers only, work
+ * (0 * inf); a row all of whose logits are -inf gives NaN and a log-sum-exp of -inf, as 0 / 0 does.  Offsets that decrease or
+ * leave [0, num_tokens] are clamped (no access outside the tensors), the results are then unspecified.  Device pointers only, work
  * is enqueued on `stream` of the current device; no state, no workspace: calls may overlap and be captured. */
 int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
                         int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v, int64_t v_token_stride,
@@ -420,7 +421,8 @@ int mp_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_hea
  * touched; in attention the latter give 0 and -inf.  A page may belong to several requests; what two rows
  * appended to one place in one call leave there is unspecified.
  * A page id outside [0, num_pages) or a kv_len outside [0, pages_per_seq * page_size] accesses nothing outside the cache: the
- * row is skipped (append, read), or the output unspecified (attention), and mp_paged_check reports it.
+ * rows of that page, all new rows of that request are skipped (append, read), or the output is unspecified (attention), and
+ * mp_paged_check reports it.
  * Tensors are bf16, 16-byte aligned, read through token and head strides that are multiples of 8 elements (token strides below 2^23;
  * dims contiguous), and written contiguously.  Device pointers only.  The handle holds the pages alone: calls that read may overlap;
  * attention's scratch memory is the caller's. */

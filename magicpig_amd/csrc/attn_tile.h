@@ -105,7 +105,8 @@ __device__ __forceinline__ bf16x8 read_v(const char* vt, int i, int t) {
 }
 
 // A masked tile may hold values that a row must not see, and 0 times an infinity is NaN.  Product with zeros first:
-// finite values give 0, anything else NaN.
+// finite values give 0, anything else NaN.  (Every row sees a tile without a mask: its values are multiplied as they are, and an
+// infinity whose weight is 0 in f32 gives NaN there, as it does where a row that holds one is scaled by 0.)
 template <int D, int SUB>
 __device__ __forceinline__ bool tile_has_nonfinite(const char* vt) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};

@@ -7,7 +7,8 @@ append, read and attention take the same description of their rows (int32 CUDA t
     cu_seqlens [B + 1]   request b's new rows in the packed tensors: cu_seqlens[b] .. cu_seqlens[b + 1]
     page_table [B, P]    position p of request b lies in page page_table[b, p // page_size]
     kv_len     [B]       positions of request b, its new rows included
-A request may have no new rows; rows outside every request, and rows whose position would be below 0, are not touched.
+A request may have no new rows; rows outside every request, rows whose position would be below 0, and the rows of a request
+whose kv_len its table cannot hold are not touched (check() reports the last).
 """
 from __future__ import annotations
 
