@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import attention64
-from magicpig_amd import decode_harness as dh
+from magicpig_amd import MagicPigError, decode_harness as dh
 from test_gpu_paged_cache import stored
 
 SHAPE = dict(num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2, intermediate_size=768, vocab_size=1000)
@@ -260,3 +260,96 @@ def test_every_dense_layer_of_decode_steps_over_pages(fmt):
             for step, (_, q, kn, vn, out) in enumerate(mine):
                 k, v = torch.cat([k, kn[r].view(1, 2, -1)]), torch.cat([v, vn[r].view(1, 2, -1)])
                 attention_is(out[r], q[r].view(1, 4, -1), stored(k, fmt), stored(v, fmt), n + step)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dense_cache", ["store", "bf16", "e4m3"])
+def test_a_request_slot_is_used_again(dense_cache):
+    """Another prompt, shorter or longer, in a slot that has served one: as in a decoder that never held the first."""
+    a, b = decoder(dense_cache=dense_cache), decoder(dense_cache=dense_cache)
+    first, second, third = prompts(700, 300, 333)
+    ids = a.prefill([first, third]).argmax(-1, keepdim=True)
+    for step in range(2):
+        a.inference(ids, torch.tensor([[700 + step], [333 + step]], device="cuda"))
+    for prompt in (second, first):
+        n = prompt.numel()
+        got, want = a.prefill([prompt, third]), b.prefill([prompt, third])
+        assert torch.equal(got, want)
+        ids, pos = want.argmax(-1, keepdim=True), torch.tensor([[n], [333]], device="cuda")
+        assert torch.equal(a.inference(ids, pos), b.inference(ids, pos))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dense_cache", ["store", "bf16"])
+def test_the_shortest_and_the_longest_prompt(dense_cache):
+    """69 tokens leave one outside the window; max_length - 1 leave room for one."""
+    dec = decoder(dense_cache=dense_cache)
+    log, _, steps = record(dec)
+    ps = prompts(69, 1023)
+    la = dec.prefill(ps)
+    for i, p in enumerate(ps):
+        close(la[i:i + 1], reference_prefill(dec, p))
+    out = dec.inference(la.argmax(-1, keepdim=True), torch.tensor([[69], [1023]], device="cuda"))
+    assert bool(torch.isfinite(out).all())
+    dec.dense_server.check()
+    dec.attention_server.window_server.check()
+    _, q, k, v, got = steps[0]
+    for r, (a, b) in enumerate(((0, 69), (69, 1092))):
+        kk, vv = (torch.cat([x[a:b], y[r].view(1, 2, -1)]) for x, y in ((log[0][3], k), (log[0][4], v)))
+        attention_is(got[r], q[r].view(1, 4, -1), kk, vv, b - a)
+
+
+@pytest.mark.gpu
+def test_prefill_on_two_ranks_is_the_unsharded_one():
+    """Two tensor-parallel ranks as two threads on one device, partial sums meeting at a barrier, against the unsharded model."""
+    import threading
+
+    one = decoder(tp_blocks=2)
+    ps = prompts(300, 71)
+    want = one.prefill(ps)
+    want_long = one.prefill_chunked(0, ps[0], chunk=128)
+    torch.cuda.synchronize()
+    meet, slot, got, errors = threading.Barrier(2, timeout=60), [None, None], [None, None], []
+
+    def run(rank):
+        def all_reduce(t):
+            slot[rank] = t
+            meet.wait()
+            total = slot[0] + slot[1]
+            meet.wait()
+            t.copy_(total)
+        try:
+            torch.cuda.set_device(0)
+            dec = decoder(tp_rank=rank, tp_world=2, all_reduce=all_reduce)
+            got[rank] = dec.prefill(ps), dec.prefill_chunked(0, ps[0], chunk=128)
+            torch.cuda.synchronize()
+        except BaseException as e:          # noqa: BLE001 -- a failing rank must not leave the other at the barrier
+            errors.append((rank, repr(e)))
+            meet.abort()
+    threads = [threading.Thread(target=run, args=(r,)) for r in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=90)
+    assert not errors, errors
+    for x, y, ref in zip(got[0], got[1], (want, want_long)):
+        assert torch.equal(x, y)
+        close(x, ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dense_cache", ["bf16", "e4m3"])
+def test_a_request_that_has_filled_its_pages(dense_cache):
+    """A step behind a prompt of max_length tokens: reported, its pages as they were; the other request goes on."""
+    dec = decoder(dense_cache=dense_cache)
+    _, _, steps = record(dec)
+    ids = dec.prefill(prompts(300, 1024)).argmax(-1, keepdim=True)
+    pages = dec.dense_server.get_pages(0)[0].view(torch.uint8)
+    before = pages.clone()
+    dec.inference(ids, torch.tensor([[300], [1023]], device="cuda"))
+    with pytest.raises(MagicPigError, match="kv_len"):
+        dec.dense_server.check()
+    page, slot = int(dec.dense_table[0, 300 // 64]), 300 % 64
+    assert not torch.equal(pages[page, :, slot], before[page, :, slot])
+    before[page, :, slot] = pages[page, :, slot]
+    assert torch.equal(pages, before)
