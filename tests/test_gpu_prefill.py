@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import attention64
-from magicpig_amd import MagicPigError, decode_harness as dh
+from magicpig_amd import decode_harness as dh
+from magicpig_amd import MagicPigError
 from test_gpu_paged_cache import stored
 
 SHAPE = dict(num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2, intermediate_size=768, vocab_size=1000)
